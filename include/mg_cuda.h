@@ -7,7 +7,9 @@
  * boundary those method bodies are replaced by.  Each entry point names the
  * reference loop it stands in for.  All pointers named `d_*`, and every
  * `double *` / `int *` argument unless marked "host", are DEVICE pointers
- * obtained from mg_alloc(); tensors are dense, row-major, fp64.
+ * obtained from mg_alloc(); tensors are dense, row-major, fp64.  (Memory of the same
+ * device from another allocator works too; its owner orders its own streams against
+ * the compute stream, with mg_sync() or by waiting before the call.)
  *
  * Conventions
  *   - Every function returns MG_OK (0) or a negative MG_ERR_* code and never
@@ -53,6 +55,7 @@ extern "C" {
 
 #define MG_ACC_STORE_A 1 /* first gradient destination is known zero  */
 #define MG_ACC_STORE_B 2 /* second gradient destination is known zero */
+#define MG_ACC_STORE_C 4 /* third gradient destination is known zero  */
 
 /* ---- lifecycle -------------------------------------------------------- */
 /* Role of the reference's MetalContext singleton
@@ -92,6 +95,8 @@ int mg_free(double *p);
 int mg_pool_reserve(size_t bytes);
 int mg_alloc_i32(size_t n, int **out);
 int mg_free_i32(int *p);
+int mg_alloc_i8(size_t n, signed char **out); /* codes of the 8-bit form (mg_q8_pack) */
+int mg_free_i8(signed char *p);
 int mg_upload(double *dst, const double *src_host, size_t n);   /* pageable or pinned host */
 int mg_download(double *dst_host, const double *src, size_t n); /* blocks until done */
 /* Prefetch: copies on a separate copy stream, so the transfer of the next batch
@@ -224,10 +229,69 @@ int mg_softmax_xent_fwd(const double *logits, const int *labels, double *loss1, 
 /* glogits[M,C] += gloss1[0] * (softmax - onehot) / denom. */
 int mg_softmax_xent_bwd(const double *logits, const int *labels, const double *gloss1,
                         double *glogits, size_t M, size_t C, double denom, int flags);
+/* The same loss of a linear layer z = x w + bias over many classes, without the
+ * M x V logits: x[M,K], w[K,V], bias[V] (NULL: none), labels[M] (int).  A row whose
+ * label is -1 is left out (a padded batch): it adds nothing to the loss or to any
+ * gradient, whatever its values are; any other label outside [0, V) is left out too
+ * and raises kernel fault 101.  loss1[0] = sum over the kept rows / denom.
+ * _fwd computes the loss alone (2 M K V flop).  _fwd_bwd also computes
+ *   gx[M,K] += gloss1[0] dloss/dx,  gw[K,V] += ...,  gbias[V] += ...
+ * in the same pass (6 M K V flop); gloss1 (one double on the device, NULL: 1) is the
+ * gradient with respect to the loss, each destination may be NULL, and
+ * MG_ACC_STORE_A / _B / _C say that gx / gw / gbias hold nothing yet.  The logits
+ * exist for a block of rows at a time, in a workspace from the pool of mg_alloc (at
+ * most 1 GiB or 128 rows).  Any K and V; odd ones, and arrays off a 16-byte boundary,
+ * are copied once into rows the tensor kernel can take. */
+int mg_linear_xent_fwd(const double *x, const double *w, const double *bias, const int *labels,
+                       double *loss1, size_t M, size_t K, size_t V, double denom);
+int mg_linear_xent_fwd_bwd(const double *x, const double *w, const double *bias, const int *labels,
+                           const double *gloss1, double *loss1, double *gx, double *gw,
+                           double *gbias, size_t M, size_t K, size_t V, double denom, int flags);
 /* First index of the strict row maximum (the `>` loop of src/main.cpp:29-32). */
 int mg_argmax_rows(const double *x, int *out, size_t M, size_t N);
 /* labels stored as doubles -> int class ids. */
 int mg_f64_to_i32(const double *src, int *dst, size_t n);
+
+/* ---- group norm with an activation (no counterpart in the reference) ----- */
+/* Channels last: x[N,P,C], N samples of P positions (P = 1 for the rows of a linear
+ * layer), C channels in G groups of neighbours.  Forward:
+ *   y = act((x - mean) rstd gamma + beta),  rstd = 1 / sqrt(var + eps)
+ * with the mean and the (biased) variance of each group's P C/G values; gamma[C] and
+ * beta[C] may be NULL (1 and 0).  mean[N,G] and rstd[N,G] are outputs and go into the
+ * backward pass. */
+enum { MG_ACT_NONE = 0, MG_ACT_RELU = 1, MG_ACT_SILU = 2 /* z / (1 + exp(-z)) */ };
+int mg_group_norm_fwd(const double *x, const double *gamma, const double *beta, double *y,
+                      double *mean, double *rstd, size_t N, size_t P, size_t C, size_t G,
+                      double eps, int act);
+/* gx += dx, ggamma[C] += ..., gbeta[C] += ... (each may be NULL); MG_ACC_STORE_A / _B /
+ * _C say that they hold nothing yet.  x is the forward input, not the output. */
+int mg_group_norm_bwd(const double *x, const double *gamma, const double *beta,
+                      const double *mean, const double *rstd, const double *gy, double *gx,
+                      double *ggamma, double *gbeta, size_t N, size_t P, size_t C, size_t G,
+                      int act, int flags);
+
+/* ---- activations kept in 8 bits (no counterpart in the reference) --------- */
+/* x[M,N] becomes codes[M,N] (one byte each) and scales[M, ceil(N / MG_Q8_BLOCK)]: a
+ * block of MG_Q8_BLOCK columns of a row shares scale = max |x| / 127, and
+ * code = rint(x / scale), except that a value that is not 0 never gets code 0.  The
+ * value kept is code * scale: at most scale away from x, at most scale / 2 where
+ * |x| >= scale / 2; and the sign of the code is always the sign of x, so a ReLU mask
+ * taken from the codes is exact.  A block whose largest magnitude is below 1e-300 is
+ * kept as zeros (the codes still hold the signs); one with an infinity or a NaN reads
+ * back as NaN.  N * M bytes of codes come from mg_alloc_i8. */
+#define MG_Q8_BLOCK 64
+int mg_q8_pack(const double *x, signed char *codes, double *scales, size_t M, size_t N);
+int mg_q8_unpack(const signed char *codes, const double *scales, double *x, size_t M, size_t N);
+/* The backward pass on the 8-bit form.  mg_gemm_tn and mg_gemm_nt with
+ * MG_EPI_RELU_MASK, their A operand / mask source in 8 bits:
+ *   dB[K,N] (+)= x[M,K]^T . G[M,N],  x = the values codes and scales keep;
+ *   dA[M,K] (+)= (G[M,N] . B[K,N]^T) * (mask_codes[M,K] > 0);
+ * and the ReLU mask alone: gx[n] += g[n] * (codes[n] > 0). */
+int mg_gemm_tn_q8(const signed char *codes, const double *scales, const double *G, double *dB,
+                  size_t M, size_t N, size_t K, int accumulate);
+int mg_gemm_nt_q8(const double *G, const double *B, double *dA, size_t M, size_t N, size_t K,
+                  int accumulate, const signed char *mask_codes);
+int mg_relu_bwd_q8(const signed char *codes, const double *g, double *gx, size_t n, int flags);
 
 /* avg_pool_2x2, src/nn.cpp:17-35, for a batch: x[batch,784] (28x28 images) ->
  * out[batch,196]; each cell is ((a+b)+c)+d over its 2x2 window, divided by 4.0. */

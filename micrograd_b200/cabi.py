@@ -21,9 +21,11 @@ _sz = C.c_size_t
 
 OK = 0
 ERR_INVALID, ERR_OOM, ERR_CUDA, ERR_NCCL, ERR_TIMEOUT, ERR_KERNEL = -1, -2, -3, -4, -5, -6
-ACC_STORE_A, ACC_STORE_B = 1, 2
+ACC_STORE_A, ACC_STORE_B, ACC_STORE_C = 1, 2, 4
 ADD, SUB, MUL, DIV = 0, 1, 2, 3
 SADD, SSUB, SMUL, SDIV, POW, RELU, SIGMOID, TANH, EXP = range(9)
+ACT_NONE, ACT_RELU, ACT_SILU = 0, 1, 2
+Q8_BLOCK = 64
 EPI_NONE, EPI_BIAS, EPI_BIAS_RELU, EPI_RELU_MASK = 0, 1, 2, 3
 
 # name -> (restype, argtypes); int-returning functions are status codes.
@@ -43,6 +45,8 @@ SIGNATURES = {
     "mg_free": (C.c_int, [C.c_void_p]),
     "mg_alloc_i32": (C.c_int, [_sz, C.POINTER(C.c_void_p)]),
     "mg_free_i32": (C.c_int, [C.c_void_p]),
+    "mg_alloc_i8": (C.c_int, [_sz, C.POINTER(C.c_void_p)]),
+    "mg_free_i8": (C.c_int, [C.c_void_p]),
     "mg_upload": (C.c_int, [C.c_void_p, C.c_void_p, _sz]),
     "mg_download": (C.c_int, [C.c_void_p, C.c_void_p, _sz]),
     "mg_upload_async": (C.c_int, [C.c_void_p, C.c_void_p, _sz, _ip]),
@@ -76,6 +80,15 @@ SIGNATURES = {
     "mg_softmax_xent_fwd": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, _sz, _sz, C.c_double]),
     "mg_softmax_xent_bwd": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, _sz, _sz,
                                       C.c_double, C.c_int]),
+    "mg_linear_xent_fwd": (C.c_int, [C.c_void_p] * 5 + [_sz, _sz, _sz, C.c_double]),
+    "mg_linear_xent_fwd_bwd": (C.c_int, [C.c_void_p] * 9 + [_sz, _sz, _sz, C.c_double, C.c_int]),
+    "mg_group_norm_fwd": (C.c_int, [C.c_void_p] * 6 + [_sz, _sz, _sz, _sz, C.c_double, C.c_int]),
+    "mg_group_norm_bwd": (C.c_int, [C.c_void_p] * 9 + [_sz, _sz, _sz, _sz, C.c_int, C.c_int]),
+    "mg_q8_pack": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, _sz, _sz]),
+    "mg_q8_unpack": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, _sz, _sz]),
+    "mg_gemm_tn_q8": (C.c_int, [C.c_void_p] * 4 + [_sz, _sz, _sz, C.c_int]),
+    "mg_gemm_nt_q8": (C.c_int, [C.c_void_p] * 3 + [_sz, _sz, _sz, C.c_int, C.c_void_p]),
+    "mg_relu_bwd_q8": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, _sz, C.c_int]),
     "mg_argmax_rows": (C.c_int, [C.c_void_p, C.c_void_p, _sz, _sz]),
     "mg_f64_to_i32": (C.c_int, [C.c_void_p, C.c_void_p, _sz]),
     "mg_avg_pool_28": (C.c_int, [C.c_void_p, C.c_void_p, _sz]),

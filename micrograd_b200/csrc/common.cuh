@@ -37,6 +37,9 @@ struct Context {
   // Split-K scratch for the transposed-A GEMM.
   double *splitk_scratch = nullptr;
   size_t splitk_scratch_elems = 0;
+  // Partial sums of the group norm kernels.
+  double *norm_scratch = nullptr;
+  size_t norm_scratch_elems = 0;
   // Kernel fault word: kernels write a non-zero code here instead of trapping.
   int *kernel_status = nullptr;        // device
   int *status_host = nullptr;          // pinned mirror of kernel_status (mg_kernel_status_mirror)

@@ -186,6 +186,7 @@ int mg_shutdown(void) {
   g_retired_scratch.clear();
   if (c.colsum_scratch) cudaFreeAsync(c.colsum_scratch, c.stream);
   if (c.splitk_scratch) cudaFreeAsync(c.splitk_scratch, c.stream);
+  if (c.norm_scratch) cudaFreeAsync(c.norm_scratch, c.stream);
   cudaStreamSynchronize(c.stream);
   gemm_release_tables();
   cudaFree(c.reduce_partials);
@@ -300,6 +301,9 @@ int mg_free(double *p) {
   }
   return MG_OK;
 }
+
+int mg_alloc_i8(size_t n, signed char **out) { return alloc_bytes(n, (void **)out); }
+int mg_free_i8(signed char *p) { return mg_free(reinterpret_cast<double *>(p)); }
 
 int mg_free_i32(int *p) { return mg_free(reinterpret_cast<double *>(p)); }
 

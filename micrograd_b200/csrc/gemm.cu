@@ -37,6 +37,7 @@
 // checks for shapes the TMA path cannot take (odd row lengths, unaligned
 // bases) and for tiny problems.
 #include "common.cuh"
+#include "gemm.cuh"
 #include "tma.cuh"
 
 #include <algorithm>
@@ -694,16 +695,6 @@ gemm_fallback_kernel(StridedOperands op, GemmEpilogue ep, int M, int N, int K) {
 // ---------------------------------------------------------------------------
 // Host dispatch
 // ---------------------------------------------------------------------------
-struct GemmDesc {
-  const double *A;  // a_kcontig ? [M][K] : [K][M]
-  const double *B;  // b_kcontig ? [N][K] : [K][N]
-  double *D;        // [M][N]
-  size_t M, N, K;
-  bool a_kcontig, b_kcontig;
-  int accumulate, mode;
-  const double *aux;
-};
-
 static int g_gemm_path = 0;    // 0 auto, 1 fallback only, 2 tensor-core whenever eligible
 static int g_dmma_shape = -1;  // -1: default
 
@@ -1027,7 +1018,7 @@ static bool dmma_eligible(const GemmDesc &d) {
   return true;
 }
 
-static int run_gemm(const GemmDesc &d) {
+int run_gemm(const GemmDesc &d) {
   if (d.M == 0 || d.N == 0) return MG_OK;
   Context &c = ctx();
   GemmEpilogue ep;
