@@ -1,0 +1,174 @@
+// The tensor-core GEMM of gemm.cu for callers whose matrices are not dense even rows:
+// see run_gemm_ext in gemm.cuh.
+#include "gemm_kernel.cuh"
+
+namespace mg {
+
+// One instantiation per tile, contraction split and grid form; all can skip the
+// ragged border (EDGE) and write any output (ANYD).
+template <bool AK, bool BK_, class Cfg, bool Q8A> static int launch_ext(const DmmaLaunch &L) {
+  if (L.tickets) return launch_dmma_masked<AK, BK_, 2, true, Cfg, false, false, true, true, Q8A>(L);
+  if (!L.table && (L.min_nkt < 32 || Cfg::BN <= 32) && L.items > ctx().sm_count)
+    return launch_dmma_masked<AK, BK_, 2, true, Cfg, true, false, false, true, Q8A>(L);
+  return launch_dmma_masked<AK, BK_, 2, true, Cfg, false, false, false, true, Q8A>(L);
+}
+
+template <bool AK, bool BK_> static int launch_layout_ext(int tile, const DmmaLaunch &L) {
+  switch (tile) {
+    case kTileSkinny: return launch_ext<AK, BK_, SkinnyCfg, false>(L);
+    case kTileSkinny16: return launch_ext<AK, BK_, Skinny16Cfg, false>(L);
+    case kTileHalf: return launch_ext<AK, BK_, HalfCfg, false>(L);
+    case kTileRows16: return launch_ext<AK, BK_, Rows16Cfg, false>(L);
+    case kTileRows32: return launch_ext<AK, BK_, Rows32Cfg, false>(L);
+    case kTileRows64: return launch_ext<AK, BK_, Rows64Cfg, false>(L);
+    default: return launch_ext<AK, BK_, MainCfg, false>(L);
+  }
+}
+
+static int launch_q8(int tile, const DmmaLaunch &L) {
+  switch (tile) {
+    case kTileSkinny: return launch_ext<false, false, SkinnyCfg, true>(L);
+    case kTileSkinny16: return launch_ext<false, false, Skinny16Cfg, true>(L);
+    case kTileHalf: return launch_ext<false, false, HalfCfg, true>(L);
+    default: return launch_ext<false, false, MainCfg, true>(L);
+  }
+}
+
+// Few rows go to tiles of few rows, unless the columns are few as well.
+static GemmPlan plan_ext(int M, int N, int K, int sms, bool q8) {
+  if (!q8 && M <= 64 && N > SkinnyCfg::BN) {
+    GemmPlan p = M <= 16 ? GemmPlan{kTileRows16, 16, 128, 0}
+                         : (M <= 32 ? GemmPlan{kTileRows32, 32, 128, 0} : GemmPlan{kTileRows64, 64, 128, 0});
+    p.spans = choose_spans((N + 127) / 128, (K + BK - 1) / BK, sms);
+    return p;
+  }
+  return choose_plan(M, N, K, sms, 2, false);
+}
+
+__global__ void __launch_bounds__(256)
+copy_rows_kernel(const double *__restrict__ src, size_t rows, size_t cols, size_t src_pitch,
+                 double *__restrict__ dst, size_t dst_pitch, const int *__restrict__ labels, size_t classes) {
+  // (threads x along the row, y over rows: short rows still fill a warp)
+  for (size_t r = (size_t)blockIdx.y * blockDim.y + threadIdx.y; r < rows; r += (size_t)gridDim.y * blockDim.y) {
+    const bool live = !labels || (labels[r] >= 0 && (size_t)labels[r] < classes);
+    for (size_t c = (size_t)blockIdx.x * blockDim.x + threadIdx.x; c < dst_pitch; c += (size_t)gridDim.x * blockDim.x)
+      dst[r * dst_pitch + c] = live && c < cols ? src[r * src_pitch + c] : 0.0;
+  }
+}
+
+int copy_rows(const double *src, size_t rows, size_t cols, size_t src_pitch, double *dst, size_t dst_pitch,
+              const int *labels, size_t classes) {
+  if (rows == 0 || dst_pitch == 0) return MG_OK;
+  unsigned x = 16;
+  while (x < 256 && x < dst_pitch) x *= 2;
+  const unsigned y = 256 / x;
+  const size_t gx = (dst_pitch + x * 4 - 1) / (x * 4);  // four columns per thread
+  size_t gy = (rows + y - 1) / y;
+  const size_t cap = (size_t)ctx().sm_count * 32 / (gx < 64 ? gx : 64) + 1;
+  if (gy > cap) gy = cap;
+  if (gy > 65535) gy = 65535;
+  copy_rows_kernel<<<dim3((unsigned)(gx < 64 ? gx : 64), (unsigned)gy), dim3(x, y), 0, ctx().stream>>>(
+      src, rows, cols, src_pitch, dst, dst_pitch, labels, classes);
+  MG_LAUNCH_CHECK("copy_rows");
+  return MG_OK;
+}
+
+__global__ void __launch_bounds__(256)
+empty_product_kernel(double *D, size_t M, size_t N, size_t ldd, int mode, const double *__restrict__ bias,
+                     int accumulate) {
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < M * N; i += (size_t)gridDim.x * 256) {
+    const size_t r = i / N, c = i - r * N;
+    double v = mode == MG_EPI_BIAS || mode == MG_EPI_BIAS_RELU ? bias[c] : 0.0;
+    if (mode == MG_EPI_BIAS_RELU) v = v > 0 ? v : 0.0;
+    D[r * ldd + c] = accumulate ? D[r * ldd + c] + v : v;
+  }
+}
+
+int run_gemm_ext(const GemmExt &e) {
+  const GemmDesc &d = e.d;
+  const bool q8 = e.codes != nullptr;
+  if (d.M == 0 || d.N == 0) return MG_OK;
+  const size_t lim = (size_t)1 << 30;
+  if (d.M >= lim || d.N >= lim || d.K >= lim) return fail(MG_ERR_INVALID, "gemm: dimension too large");
+  const size_t a_row = d.a_kcontig ? d.K : d.M, b_row = d.b_kcontig ? d.K : d.N;
+  const size_t lda = e.lda ? e.lda : a_row, ldb = e.ldb ? e.ldb : b_row, ldd = e.ldd ? e.ldd : d.N;
+  const bool dense = lda == a_row && ldb == b_row && ldd == d.N && !((a_row | b_row | d.N) & 1) &&
+                     !off_16_bytes(d.D);
+  if (d.K == 0) {
+    // Nothing to sum up (and no tensor map of nothing): the epilogue alone.
+    if (d.accumulate && d.mode == MG_EPI_NONE) return MG_OK;
+    empty_product_kernel<<<grid_for(d.M * d.N, 256, 16), 256, 0, ctx().stream>>>(d.D, d.M, d.N, ldd, d.mode, d.aux,
+                                                                               d.accumulate);
+    MG_LAUNCH_CHECK("gemm (empty contraction)");
+    return MG_OK;
+  }
+  if (!q8 && !e.mask8 && dense && (d.M > 64 || d.N <= (size_t)SkinnyCfg::BN)) return run_gemm(d);
+  if ((!q8 && ((lda & 1) || off_16_bytes(d.A))) || (ldb & 1) || off_16_bytes(d.B))
+    return fail(MG_ERR_INVALID, "gemm: operand rows do not start on 16-byte boundaries");
+  Context &c = ctx();
+  const int M = (int)d.M, N = (int)d.N, K = (int)d.K;
+  const GemmPlan plan = plan_ext(M, N, K, c.sm_count, q8);
+  DmmaLaunch L{};
+  bool ok_a = true, ok_b;
+  if (q8) {
+    L.qa.codes = e.codes;
+    L.qa.scales = e.scales;
+    L.qa.ldc = lda;
+    L.qa.blocks = (d.M + MG_Q8_BLOCK - 1) / MG_Q8_BLOCK;
+    L.qa.cols = M;
+    L.qa.wide = lda % 16 == 0 && !off_16_bytes(e.codes);
+  } else if (d.a_kcontig) {
+    ok_a = make_tensor_map_f64(&L.ma, d.A, d.M, d.K, BK, plan.bm, lda);
+  } else if (lda % 16 == 0 && make_tensor_map_f64_grouped(&L.ma, d.A, d.K, lda, BK, plan.bm / 16)) {
+    L.grouped_ab |= 1;
+  } else {
+    ok_a = make_tensor_map_f64(&L.ma, d.A, d.K, d.M, 16, BK, lda);
+  }
+  if (d.b_kcontig) {
+    ok_b = make_tensor_map_f64(&L.mb, d.B, d.N, d.K, BK, plan.bn, ldb);
+  } else if (ldb % 16 == 0 && make_tensor_map_f64_grouped(&L.mb, d.B, d.K, ldb, BK, plan.bn / 16)) {
+    ok_b = true;
+    L.grouped_ab |= 2;
+  } else {
+    ok_b = make_tensor_map_f64(&L.mb, d.B, d.K, d.N, 16, BK, ldb);
+  }
+  if (!ok_a || !ok_b) return fail(MG_ERR_CUDA, "gemm: cuTensorMapEncodeTiled failed");
+  if (q8) L.ma = L.mb;
+  L.mmask = L.mb;
+
+  GemmEpilogue ep{};
+  ep.D = d.D;
+  ep.aux = d.aux;
+  ep.mode = d.mode;
+  ep.accumulate = d.accumulate;
+  ep.ldd = ldd;
+  ep.mask8 = e.mask8;
+  ep.ld_mask8 = d.N;
+  ep.pairs = ldd % 2 == 0 && !off_16_bytes(d.D);
+  const int tiles_m = (M + plan.bm - 1) / plan.bm, tiles_n = (N + plan.bn - 1) / plan.bn;
+  const int KT = (K + BK - 1) / BK;
+  const SegTable *table = nullptr;
+  if (plan.spans > 0) {
+    int rc = seg_table_for(tiles_m, tiles_n, KT, plan.bm, plan.bn, plan.spans, &table);
+    if (rc != MG_OK) return rc;
+    if (table->slots > 0) {
+      rc = ensure_scratch(&c.splitk_scratch, &c.splitk_scratch_elems,
+                          (size_t)table->slots * (size_t)plan.bm * (size_t)plan.bn);
+      if (rc != MG_OK) return rc;
+      ep.partial = c.splitk_scratch;
+    }
+  }
+  L.ep = ep;
+  L.M = M; L.N = N; L.K = K;
+  L.tiles_m = tiles_m; L.tiles_n = tiles_n;
+  L.table = table ? table->dev_items : nullptr;
+  L.tickets = table && table->slots > 0 ? table->dev_tickets : nullptr;
+  L.items = table ? table->items : tiles_m * tiles_n;
+  L.min_nkt = table ? table->min_nkt : KT;
+  if (q8) return launch_q8(plan.tile, L);
+  if (d.a_kcontig && !d.b_kcontig) return launch_layout_ext<true, false>(plan.tile, L);
+  if (d.a_kcontig) return launch_layout_ext<true, true>(plan.tile, L);
+  return launch_layout_ext<false, false>(plan.tile, L);
+}
+
+}  // namespace mg

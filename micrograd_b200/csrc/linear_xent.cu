@@ -85,36 +85,40 @@ xent_loss_kernel(const double *__restrict__ row_loss, size_t M, double inv_denom
   if (threadIdx.x == 0) loss[0] = sum * inv_denom;
 }
 
-// dst[drows][dcols] = src[srows][scols] with zeros around it; where labels are given,
-// rows that are left out become zeros too (0 times whatever they hold would not).
-__global__ void __launch_bounds__(256)
-pad_kernel(const double *__restrict__ src, size_t srows, size_t scols, double *__restrict__ dst, size_t drows,
-           size_t dcols, const int *__restrict__ labels, size_t V) {
-  for (size_t r = blockIdx.y; r < drows; r += gridDim.y) {
-    const bool live = r < srows && (!labels || (labels[r] >= 0 && (size_t)labels[r] < V));
-    for (size_t c = (size_t)blockIdx.x * 256 + threadIdx.x; c < dcols; c += (size_t)gridDim.x * 256)
-      dst[r * dcols + c] = live && c < scols ? src[r * scols + c] : 0.0;
+// out[v] (+)= sum over the rows of p[rows][pitch]: a CTA per 64 columns, its warps the
+// rows in turn (fixed order).
+constexpr int kColWarps = 16;
+__global__ void __launch_bounds__(32 * kColWarps)
+column_sums_kernel(const double *__restrict__ p, size_t pitch, size_t rows, size_t V, double *out, bool accumulate) {
+  __shared__ double part[kColWarps][64];
+  const int lane = threadIdx.x, warp = threadIdx.y;
+  const size_t c0 = (size_t)blockIdx.x * 64 + 2 * lane;
+  double s0 = 0.0, s1 = 0.0;
+  if (c0 < V) {  // (the row's last pair may reach into the pitch, which is a multiple of 16)
+#pragma unroll 4
+    for (size_t r = warp; r < rows; r += kColWarps) {
+      const double2 v = __ldcs(reinterpret_cast<const double2 *>(p + r * pitch + c0));
+      s0 += v.x;
+      s1 += v.y;
+    }
+  }
+  part[warp][2 * lane] = s0;
+  part[warp][2 * lane + 1] = s1;
+  __syncthreads();
+  const int t = warp * 32 + lane;
+  const size_t c = (size_t)blockIdx.x * 64 + t;
+  if (t < 64 && c < V) {
+    double s = 0.0;
+    for (int w = 0; w < kColWarps; w++) s += part[w][t];
+    out[c] = accumulate ? out[c] + s : s;
   }
 }
 
-// dst[rows][cols] (+)= the left part of src[rows][pitch].
-__global__ void __launch_bounds__(256)
-unpad_kernel(const double *__restrict__ src, size_t pitch, double *dst, size_t rows, size_t cols, bool accumulate) {
-  for (size_t r = blockIdx.y; r < rows; r += gridDim.y)
-    for (size_t c = (size_t)blockIdx.x * 256 + threadIdx.x; c < cols; c += (size_t)gridDim.x * 256) {
-      const double v = src[r * pitch + c];
-      dst[r * cols + c] = accumulate ? dst[r * cols + c] + v : v;
-    }
+static int column_sums(const double *p, size_t pitch, size_t rows, size_t V, double *out, bool accumulate) {
+  column_sums_kernel<<<(unsigned)((V + 63) / 64), dim3(32, kColWarps), 0, ctx().stream>>>(p, pitch, rows, V, out, accumulate);
+  MG_LAUNCH_CHECK("linear_xent column sums");
+  return MG_OK;
 }
-
-static dim3 grid2d(size_t rows, size_t cols) {
-  const size_t gx = (cols + 255) / 256 < 64 ? (cols + 255) / 256 : 64;
-  size_t gy = rows < 65535 ? rows : 65535;
-  return dim3((unsigned)(gx ? gx : 1), (unsigned)(gy ? gy : 1));
-}
-
-static bool odd_address(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
-static size_t even(size_t n) { return (n + 1) / 2 * 2; }
 
 struct Head {
   const double *x, *w, *bias;
@@ -129,17 +133,14 @@ struct Head {
 
 static int run_head(const Head &h) {
   Context &c = ctx();
-  const bool want_gx = h.grad && h.gx, want_gw = h.grad && h.gw, want_gb = h.grad && h.gbias;
-  // The tensor kernel takes rows of an even number of doubles from 16-byte
-  // boundaries.  What does not come like that is copied into that form: M K + K V
-  // elements once, against 2 M K V flop or more.
-  const size_t Kp = even(h.K), Vp = even(h.V);
-  const bool pad_w = Kp != h.K || Vp != h.V || odd_address(h.w);
-  const bool pad_bias = h.bias && (Vp != h.V || odd_address(h.bias));
-  const bool pad_gw = want_gw && (Kp != h.K || Vp != h.V || odd_address(h.gw));
-  const bool pad_gx = want_gx && (Kp != h.K || odd_address(h.gx));
-  const bool pad_gb = want_gb && Vp != h.V;
-  const bool pad_x = h.grad || Kp != h.K || odd_address(h.x);
+  // The tensor kernel takes operand rows of an even number of doubles from 16-byte
+  // boundaries.  x and w that do not come like that are copied into rows that do (M K
+  // or K V elements once, against 2 M K V flop or more); with gradients x is copied in
+  // any case, the rows that are left out as zeros: whatever they hold, 0 times it is
+  // not 0 in x^T p.
+  const size_t Kp = pitch16(h.K), Vp = pitch16(h.V);
+  const bool copy_w = h.V % 2 != 0 || off_16_bytes(h.w);
+  const bool copy_x = h.grad || h.K % 2 != 0 || off_16_bytes(h.x);
   size_t R = kBlockBytes / sizeof(double) / Vp / 128 * 128;
   if (R < 128) R = 128;
   if (R > h.M) R = h.M;
@@ -150,41 +151,34 @@ static int run_head(const Head &h) {
     if (wanted) need += (n + 31) / 32 * 32;  // 256-byte boundaries
     return at;
   };
-  const size_t at_z = take(true, R * Vp), at_loss = take(true, h.M), at_x = take(pad_x, h.M * Kp);
-  const size_t at_w = take(pad_w, Kp * Vp), at_b = take(pad_bias, Vp), at_gw = take(pad_gw, Kp * Vp);
-  const size_t at_gx = take(pad_gx, R * Kp), at_gb = take(pad_gb, Vp);
+  const size_t at_z = take(true, R * Vp), at_loss = take(true, h.M), at_x = take(copy_x, h.M * Kp);
+  const size_t at_w = take(copy_w, h.K * Vp);
   double *ws = nullptr;
   int rc = mg_alloc(need, &ws);
   if (rc != MG_OK) return rc;
 
   rc = [&]() -> int {
-    const double *x = h.x, *w = h.w, *bias = h.bias;
-    auto pad = [&](const double *src, size_t srows, size_t scols, double *dst, size_t drows, size_t dcols,
-                   const int *labels) -> int {
-      pad_kernel<<<grid2d(drows, dcols), 256, 0, c.stream>>>(src, srows, scols, dst, drows, dcols, labels, h.V);
-      MG_LAUNCH_CHECK("linear_xent pad");
-      return MG_OK;
-    };
+    const double *x = h.x, *w = h.w;
+    const size_t ldx = copy_x ? Kp : h.K, ldw = copy_w ? Vp : h.V;
     int r;
-    if (pad_x) {
-      if ((r = pad(h.x, h.M, h.K, ws + at_x, h.M, Kp, h.grad ? h.labels : nullptr)) != MG_OK) return r;
+    if (copy_x) {
+      if ((r = copy_rows(h.x, h.M, h.K, h.K, ws + at_x, Kp, h.grad ? h.labels : nullptr, h.V)) != MG_OK) return r;
       x = ws + at_x;
     }
-    if (pad_w) {
-      if ((r = pad(h.w, h.K, h.V, ws + at_w, Kp, Vp, nullptr)) != MG_OK) return r;
+    if (copy_w) {
+      if ((r = copy_rows(h.w, h.K, h.V, h.V, ws + at_w, Vp)) != MG_OK) return r;
       w = ws + at_w;
     }
-    if (pad_bias) {
-      if ((r = pad(h.bias, 1, h.V, ws + at_b, 1, Vp, nullptr)) != MG_OK) return r;
-      bias = ws + at_b;
-    }
-    double *z = ws + at_z, *gw = pad_gw ? ws + at_gw : h.gw, *gb = pad_gb ? ws + at_gb : h.gbias;
+    double *z = ws + at_z;
     const double inv = 1.0 / h.denom;
     for (size_t m0 = 0; m0 < h.M; m0 += R) {
       const size_t rows = h.M - m0 < R ? h.M - m0 : R;
-      const double *xb = x + m0 * Kp;
-      if ((r = run_gemm({xb, w, z, rows, Vp, Kp, true, false, 0, bias ? MG_EPI_BIAS : MG_EPI_NONE, bias})) != MG_OK)
-        return r;
+      const double *xb = x + m0 * ldx;
+      GemmExt fwd{{xb, w, z, rows, h.V, h.K, true, false, 0, h.bias ? MG_EPI_BIAS : MG_EPI_NONE, h.bias}};
+      fwd.lda = ldx;
+      fwd.ldb = ldw;
+      fwd.ldd = Vp;
+      if ((r = run_gemm_ext(fwd)) != MG_OK) return r;
       if (h.grad)
         xent_rows_kernel<true><<<(unsigned)rows, kXentThreads, 0, c.stream>>>(
             z, h.labels + m0, h.gloss, ws + at_loss + m0, h.V, Vp, inv, c.kernel_status);
@@ -192,33 +186,22 @@ static int run_head(const Head &h) {
         xent_rows_kernel<false><<<(unsigned)rows, kXentThreads, 0, c.stream>>>(
             z, h.labels + m0, h.gloss, ws + at_loss + m0, h.V, Vp, inv, c.kernel_status);
       MG_LAUNCH_CHECK("linear_xent rows");
-      if (want_gx) {
-        const bool acc = !(h.flags & MG_ACC_STORE_A);
-        double *dst = pad_gx ? ws + at_gx : h.gx + m0 * h.K;
-        if ((r = run_gemm({z, w, dst, rows, Kp, Vp, true, true, pad_gx ? 0 : acc, MG_EPI_NONE, nullptr})) != MG_OK)
-          return r;
-        if (pad_gx) {
-          unpad_kernel<<<grid2d(rows, h.K), 256, 0, c.stream>>>(dst, Kp, h.gx + m0 * h.K, rows, h.K, acc);
-          MG_LAUNCH_CHECK("linear_xent gx");
-        }
-      }
       const bool first = m0 == 0;
-      if (want_gw) {
-        const bool acc = !first || (!pad_gw && !(h.flags & MG_ACC_STORE_B));
-        if ((r = run_gemm({xb, z, gw, Kp, Vp, rows, false, false, acc, MG_EPI_NONE, nullptr})) != MG_OK) return r;
+      if (h.grad && h.gx) {
+        GemmExt e{{z, w, h.gx + m0 * h.K, rows, h.K, h.V, true, true, !(h.flags & MG_ACC_STORE_A), MG_EPI_NONE, nullptr}};
+        e.lda = Vp;
+        e.ldb = ldw;
+        if ((r = run_gemm_ext(e)) != MG_OK) return r;
       }
-      if (want_gb) {
-        const bool acc = !first || (!pad_gb && !(h.flags & MG_ACC_STORE_C));
-        if ((r = mg_add_row_bwd(z, nullptr, gb, rows, Vp, acc ? 0 : MG_ACC_STORE_B)) != MG_OK) return r;
+      if (h.grad && h.gw) {
+        GemmExt e{{xb, z, h.gw, h.K, h.V, rows, false, false, !first || !(h.flags & MG_ACC_STORE_B), MG_EPI_NONE, nullptr}};
+        e.lda = ldx;
+        e.ldb = Vp;
+        if ((r = run_gemm_ext(e)) != MG_OK) return r;
       }
-    }
-    if (pad_gw) {
-      unpad_kernel<<<grid2d(h.K, h.V), 256, 0, c.stream>>>(gw, Vp, h.gw, h.K, h.V, !(h.flags & MG_ACC_STORE_B));
-      MG_LAUNCH_CHECK("linear_xent gw");
-    }
-    if (pad_gb) {
-      unpad_kernel<<<grid2d(1, h.V), 256, 0, c.stream>>>(gb, Vp, h.gbias, 1, h.V, !(h.flags & MG_ACC_STORE_C));
-      MG_LAUNCH_CHECK("linear_xent gbias");
+      if (h.grad && h.gbias) {
+        if ((r = column_sums(z, Vp, rows, h.V, h.gbias, !first || !(h.flags & MG_ACC_STORE_C))) != MG_OK) return r;
+      }
     }
     xent_loss_kernel<<<1, 1024, 0, c.stream>>>(ws + at_loss, h.M, inv, h.loss);
     MG_LAUNCH_CHECK("linear_xent loss");

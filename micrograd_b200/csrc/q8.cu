@@ -139,12 +139,20 @@ int mg_gemm_tn_q8(const signed char *codes, const double *scales, const double *
     return fail(MG_ERR_INVALID, "mg_gemm_tn_q8: null pointer");
   MG_ENSURE_INIT();
   if (K == 0 || N == 0) return MG_OK;
-  double *x = nullptr;
-  rc = mg_alloc(M * K, &x);
+  // Output [K][N], contraction over the M rows; the codes are widened inside the kernel.
+  GemmExt e{{nullptr, G, dB, K, N, M, false, false, accumulate, MG_EPI_NONE, nullptr}};
+  e.codes = codes;
+  e.scales = scales;
+  if (N % 2 == 0 && !off_16_bytes(G)) return run_gemm_ext(e);
+  // Rows of G that the tensor kernel cannot take are copied into rows it can.
+  double *g = nullptr;
+  e.ldb = pitch16(N);
+  rc = mg_alloc(M * e.ldb, &g);
   if (rc != MG_OK) return rc;
-  rc = mg_q8_unpack(codes, scales, x, M, K);
-  if (rc == MG_OK) rc = mg_gemm_tn(x, G, dB, M, N, K, accumulate);
-  const int freed = mg_free(x);
+  rc = copy_rows(G, M, N, N, g, e.ldb);
+  e.d.B = g;
+  if (rc == MG_OK) rc = run_gemm_ext(e);
+  const int freed = mg_free(g);
   return rc != MG_OK ? rc : freed;
 }
 
@@ -154,16 +162,21 @@ int mg_gemm_nt_q8(const double *G, const double *B, double *dA, size_t M, size_t
     return fail(MG_ERR_INVALID, "mg_gemm_nt_q8: null pointer");
   MG_ENSURE_INIT();
   if (M == 0 || K == 0) return MG_OK;
-  if (!accumulate) {
-    int rc = mg_gemm_nt(G, B, dA, M, N, K, 0, MG_EPI_NONE, nullptr);
-    return rc != MG_OK ? rc : mg_relu_bwd_q8(mask_codes, dA, dA, M * K, MG_ACC_STORE_A);
-  }
-  double *product = nullptr;
-  int rc = mg_alloc(M * K, &product);
+  // Output [M][K], contraction over N.
+  GemmExt e{{G, B, dA, M, K, N, true, true, accumulate, MG_EPI_NONE, nullptr}};
+  e.mask8 = mask_codes;
+  if (N % 2 == 0 && !off_16_bytes(G) && !off_16_bytes(B)) return run_gemm_ext(e);
+  const size_t pitch = pitch16(N);
+  double *room = nullptr;
+  int rc = mg_alloc((M + K) * pitch, &room);
   if (rc != MG_OK) return rc;
-  rc = mg_gemm_nt(G, B, product, M, N, K, 0, MG_EPI_NONE, nullptr);
-  if (rc == MG_OK) rc = mg_relu_bwd_q8(mask_codes, product, dA, M * K, 0);
-  const int freed = mg_free(product);
+  rc = copy_rows(G, M, N, N, room, pitch);
+  if (rc == MG_OK) rc = copy_rows(B, K, N, N, room + M * pitch, pitch);
+  e.d.A = room;
+  e.d.B = room + M * pitch;
+  e.lda = e.ldb = pitch;
+  if (rc == MG_OK) rc = run_gemm_ext(e);
+  const int freed = mg_free(room);
   return rc != MG_OK ? rc : freed;
 }
 

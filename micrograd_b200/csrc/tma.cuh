@@ -37,13 +37,14 @@ inline EncodeTiledFn encode_tiled_fn() {
 // Row-major fp64 matrix [rows][cols] viewed as a 2-D tensor (x = column,
 // y = row), copied in boxes of box_cols x box_rows with the 128-byte swizzle
 // (16-byte chunk index XOR row index mod 8).  Out-of-range elements read as 0.
-// Requirements: base 16-byte aligned, cols even, box_cols * 8 <= 128.
+// Requirements: base 16-byte aligned, row pitch (cols, unless given) even,
+// box_cols * 8 <= 128.
 inline bool make_tensor_map_f64(CUtensorMap *map, const double *base, size_t rows, size_t cols,
-                                unsigned box_cols, unsigned box_rows) {
+                                unsigned box_cols, unsigned box_rows, size_t pitch = 0) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (!fn) return false;
   cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)cols * sizeof(double)};
+  cuuint64_t strides[1] = {(cuuint64_t)(pitch ? pitch : cols) * sizeof(double)};
   cuuint32_t box[2] = {box_cols, box_rows};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT64, 2, const_cast<double *>(base), dims,
