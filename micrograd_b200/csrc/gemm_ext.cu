@@ -144,7 +144,7 @@ int run_gemm_ext(const GemmExt &e) {
   ep.ldd = ldd;
   ep.mask8 = e.mask8;
   ep.ld_mask8 = d.N;
-  ep.pairs = ldd % 2 == 0 && !off_16_bytes(d.D);
+  ep.pairs = ldd % 2 == 0 && !off_16_bytes(d.D) && !(reinterpret_cast<uintptr_t>(e.mask8) & 1);
   const int tiles_m = (M + plan.bm - 1) / plan.bm, tiles_n = (N + plan.bn - 1) / plan.bn;
   const int KT = (K + BK - 1) / BK;
   const SegTable *table = nullptr;

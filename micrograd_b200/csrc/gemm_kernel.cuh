@@ -93,6 +93,13 @@ struct Q8Operand {
   int wide;  // 16 codes can be read at once: base and pitch are multiples of 16 bytes
 };
 
+// Byte e of a word of codes, each with its top bit flipped (0 .. 255 for -128 .. 127), as
+// a double: the byte becomes the low end of 2^52 + byte, from which 2^52 + 128 is taken.
+// (An int to double conversion has a sixteenth of that rate.)
+__device__ __forceinline__ double widen_code(unsigned flipped, int e) {
+  return __hiloint2double(0x43300000, (int)__byte_perm(flipped, 0, 0x4440 + e)) - 4503599627370624.0;
+}
+
 // Fragment pair (k = 2c, 2c+1) of the A operand for the MT row sub-tiles of a
 // warp: lo = rows g, hi = rows g + 8 of each 16-row sub-tile.
 template <bool KCONTIG, int MT>
@@ -312,7 +319,7 @@ dmma_gemm_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant
   if (threadIdx.x == 0) {
     abort_flag_s = 0;
     for (int s = 0; s < kStages; s++) {
-      mbar_init(smem_u32(full_bar + s), Q8A ? 1 + kProducerWarps * 32 : 1);
+      mbar_init(smem_u32(full_bar + s), Q8A ? 1 + kProducerWarps : 1);
       mbar_init(smem_u32(empty_bar + s), kConsumerWarps);
     }
     mbar_init(smem_u32(fold_bar), kConsumerWarps);
@@ -380,15 +387,15 @@ dmma_gemm_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant
                   }
                 }
                 uint8_t *dst = stage + j * 2048 + r * 128;
-                const int word[4] = {code[u].x, code[u].y, code[u].z, code[u].w};
+                const unsigned word[4] = {(unsigned)code[u].x ^ 0x80808080u, (unsigned)code[u].y ^ 0x80808080u,
+                                          (unsigned)code[u].z ^ 0x80808080u, (unsigned)code[u].w ^ 0x80808080u};
 #pragma unroll
-                for (int c = 0; c < 8; c++) {
-                  const int two = word[c >> 1] >> (16 * (c & 1));
-                  const double lo = (double)(signed char)two * scale[u];
-                  const double hi = (double)(signed char)(two >> 8) * scale[u];
-                  *reinterpret_cast<double2 *>(dst + ((c ^ (r & 7)) << 4)) = make_double2(lo, hi);
-                }
-                mbar_arrive(bar);
+                for (int c = 0; c < 8; c++)
+                  *reinterpret_cast<double2 *>(dst + ((c ^ (r & 7)) << 4)) =
+                      make_double2(widen_code(word[c >> 1], 2 * (c & 1)) * scale[u],
+                                   widen_code(word[c >> 1], 2 * (c & 1) + 1) * scale[u]);
+                __syncwarp();
+                if ((pt & 31) == 0) mbar_arrive(bar);
                 ring++;
                 read(it + kAhead, code[u], scale[u]);
               }
@@ -586,58 +593,79 @@ dmma_gemm_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant
           bias[nt] = make_double2(use_bias && col < N ? __ldg(ep.aux + col) : 0.0,
                                   use_bias && col + 1 < N ? __ldg(ep.aux + col + 1) : 0.0);
         }
+        // Whole pairs in one access each where every pair of the output (and of the mask)
+        // starts on its own boundary, single elements otherwise.
+        const bool pairs = ep.pairs && !(N & 1);
+        constexpr int EG = (MT * NT <= 8) ? MT : 1;  // as below: small tiles fetch everything first
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
-          double2 old[2][NT];
-          bool pass[2][NT][2];
+        for (int mt0 = 0; mt0 < MT; mt0 += EG) {
+          double2 old[EG][2][NT];
+          unsigned short codes[EG][2][NT];
+          if (ep.accumulate || ep.mask8) {
 #pragma unroll
-          for (int h = 0; h < 2; h++) {
-            const int row = m0 + wm + mt * 16 + g + 8 * h;
+            for (int e = 0; e < EG; e++) {
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-              const int col = n0 + wn + nt * 8 + 2 * t;
-              const bool in0 = row < M && col < N, in1 = row < M && col + 1 < N;
-              const double *src = ep.D + (size_t)row * ep.ldd + col;
-              old[h][nt] = make_double2(0.0, 0.0);
-              if (ep.accumulate) {
-                if (in0) old[h][nt].x = __ldcs(src);
-                if (in1) old[h][nt].y = __ldcs(src + 1);
-              }
-              pass[h][nt][0] = pass[h][nt][1] = true;
-              if (ep.mask8) {
-                const signed char *m = ep.mask8 + (size_t)row * ep.ld_mask8 + col;
-                if (in0) pass[h][nt][0] = m[0] > 0;
-                if (in1) pass[h][nt][1] = m[1] > 0;
+              for (int h = 0; h < 2; h++) {
+                const int row = m0 + wm + (mt0 + e) * 16 + g + 8 * h;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                  const int col = n0 + wn + nt * 8 + 2 * t;
+                  const bool in0 = row < M && col < N, in1 = row < M && col + 1 < N;
+                  old[e][h][nt] = make_double2(0.0, 0.0);
+                  codes[e][h][nt] = 0;
+                  if (ep.mask8) {
+                    const signed char *m = ep.mask8 + (size_t)row * ep.ld_mask8 + col;
+                    if (pairs) {
+                      if (in0) codes[e][h][nt] = __ldg(reinterpret_cast<const unsigned short *>(m));
+                    } else {
+                      if (in0) codes[e][h][nt] = (unsigned char)m[0];
+                      if (in1) codes[e][h][nt] |= (unsigned short)((unsigned char)m[1] << 8);
+                    }
+                  }
+                  if (ep.accumulate) {
+                    const double *src = ep.D + (size_t)row * ep.ldd + col;
+                    if (pairs) {
+                      if (in0) old[e][h][nt] = __ldcs(reinterpret_cast<const double2 *>(src));
+                    } else {
+                      if (in0) old[e][h][nt].x = __ldcs(src);
+                      if (in1) old[e][h][nt].y = __ldcs(src + 1);
+                    }
+                  }
+                }
               }
             }
           }
 #pragma unroll
-          for (int h = 0; h < 2; h++) {
-            const int row = m0 + wm + mt * 16 + g + 8 * h;
-            if (row >= M) continue;
+          for (int e = 0; e < EG; e++) {
+            const int mt = mt0 + e;
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-              const int col = n0 + wn + nt * 8 + 2 * t;
-              if (col >= N) continue;
-              double2 v = make_double2(acc[mt][nt][2 * h] + bias[nt].x, acc[mt][nt][2 * h + 1] + bias[nt].y);
-              if (ep.mode == MG_EPI_BIAS_RELU) {
-                v.x = v.x > 0 ? v.x : 0.0;
-                v.y = v.y > 0 ? v.y : 0.0;
-              }
-              if (ep.mask8) {
-                v.x = v.x * (pass[h][nt][0] ? 1.0 : 0.0);
-                v.y = v.y * (pass[h][nt][1] ? 1.0 : 0.0);
-              }
-              if (ep.accumulate) {
-                v.x = old[h][nt].x + v.x;
-                v.y = old[h][nt].y + v.y;
-              }
-              double *dst = ep.D + (size_t)row * ep.ldd + col;
-              if (ep.pairs && col + 1 < N) {
-                *reinterpret_cast<double2 *>(dst) = v;
-              } else {
-                dst[0] = v.x;
-                if (col + 1 < N) dst[1] = v.y;
+            for (int h = 0; h < 2; h++) {
+              const int row = m0 + wm + mt * 16 + g + 8 * h;
+              if (row >= M) continue;
+#pragma unroll
+              for (int nt = 0; nt < NT; nt++) {
+                const int col = n0 + wn + nt * 8 + 2 * t;
+                if (col >= N) continue;
+                double2 v = make_double2(acc[mt][nt][2 * h] + bias[nt].x, acc[mt][nt][2 * h + 1] + bias[nt].y);
+                if (ep.mode == MG_EPI_BIAS_RELU) {
+                  v.x = v.x > 0 ? v.x : 0.0;
+                  v.y = v.y > 0 ? v.y : 0.0;
+                }
+                if (ep.mask8) {
+                  v.x = v.x * ((signed char)codes[e][h][nt] > 0 ? 1.0 : 0.0);
+                  v.y = v.y * ((short)codes[e][h][nt] >= 256 ? 1.0 : 0.0);  // (its high byte > 0)
+                }
+                if (ep.accumulate) {
+                  v.x = old[e][h][nt].x + v.x;
+                  v.y = old[e][h][nt].y + v.y;
+                }
+                double *dst = ep.D + (size_t)row * ep.ldd + col;
+                if (ep.pairs && col + 1 < N) {
+                  *reinterpret_cast<double2 *>(dst) = v;
+                } else {
+                  dst[0] = v.x;
+                  if (col + 1 < N) dst[1] = v.y;
+                }
               }
             }
           }

@@ -15,11 +15,12 @@
 #include "common.cuh"
 #include "gemm.cuh"
 
+#include <cooperative_groups.h>
+
 namespace mg {
 
 // Logits held at a time.
 constexpr size_t kBlockBytes = (size_t)1 << 30;
-constexpr int kXentThreads = 256;
 
 __device__ __forceinline__ double block_reduce(double v, bool take_max, double *smem32) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -41,38 +42,194 @@ __device__ __forceinline__ double block_reduce(double v, bool take_max, double *
   return v;
 }
 
-// A CTA per row of the block: row_loss[i], and the row's logits replaced by p (with
-// zeros in the columns from V to pitch) when GRAD.
-template <bool GRAD>
-__global__ void __launch_bounds__(kXentThreads)
+// Over the CS CTAs of a row; slot is double-buffered by the two calls a row makes.
+template <int CS> __device__ __forceinline__ double row_reduce(double v, bool take_max, double *smem32, double *slot) {
+  v = block_reduce(v, take_max, smem32);
+  if (CS == 1) return v;
+  auto cluster = cooperative_groups::this_cluster();
+  if (threadIdx.x == 0) *slot = v;
+  cluster.sync();
+  double all = take_max ? -INFINITY : 0.0;
+#pragma unroll
+  for (int r = 0; r < CS; r++) {
+    const double o = *cluster.map_shared_rank(slot, r);
+    all = take_max ? fmax(all, o) : all + o;
+  }
+  return all;
+}
+
+// A row's loss and, when GRAD, its logits replaced by p.  CS CTAs (a cluster) share a
+// row: each keeps its part, a contiguous piece of `piece` classes (a multiple of 4, at
+// most kRowsThreads x kRowsValues), in registers, so that a logit is read once, its
+// exponential computed once and p written once.  What is between V and the pitch is
+// neither used nor written.
+constexpr int kRowsThreads = 512, kRowsValues = 16;
+
+template <bool GRAD, int CS>
+__global__ void __launch_bounds__(kRowsThreads, 2)
 xent_rows_kernel(double *__restrict__ z, const int *__restrict__ labels, const double *__restrict__ gloss,
-                 double *__restrict__ row_loss, size_t V, size_t pitch, double inv_denom, int *status) {
+                 double *__restrict__ row_loss, int V, size_t pitch, int piece, double inv_denom, int *status) {
+  __shared__ double smem32[32];
+  __shared__ double slot[2];
+  const size_t row = blockIdx.x / CS;
+  const int rank = CS > 1 ? (int)(blockIdx.x % CS) : 0;
+  const int begin = rank * piece, end = begin + piece < V ? begin + piece : V;
+  double *r = z + row * pitch;
+  const int label = labels[row];
+  const bool keep = label >= 0 && label < V;
+  if (!keep) {  // (the same in all CTAs of the row)
+    if (threadIdx.x == 0 && rank == 0) {
+      if (label != -1) atomicExch(status, 101);  // not a class and not "left out"
+      row_loss[row] = 0.0;
+    }
+    if (GRAD)
+      for (int j = begin + threadIdx.x; j < end; j += kRowsThreads) r[j] = 0.0;
+    return;
+  }
+  double v[kRowsValues];
+  double top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kRowsValues / 4; i++) {
+    const int j = begin + (i * kRowsThreads + threadIdx.x) * 4;
+    double4v q{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    if (j < end) q = *reinterpret_cast<const double4v *>(r + j);  // (the pitch is a multiple of 16)
+    v[4 * i] = q.x;
+    v[4 * i + 1] = j + 1 < end ? q.y : -INFINITY;
+    v[4 * i + 2] = j + 2 < end ? q.z : -INFINITY;
+    v[4 * i + 3] = j + 3 < end ? q.w : -INFINITY;
+  }
+#pragma unroll
+  for (int i = 0; i < kRowsValues; i++) top = fmax(top, v[i]);
+  top = row_reduce<CS>(top, true, smem32, &slot[0]);
+  const double at_label = threadIdx.x == 0 && rank == 0 ? r[label] : 0.0;
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < kRowsValues; i++) {
+    const int j = begin + ((i >> 2) * kRowsThreads + threadIdx.x) * 4 + (i & 3);
+    if (j < end) {
+      v[i] = exp(v[i] - top);
+      sum += v[i];
+    }
+  }
+  // (p is written only after every CTA of the row has passed this meeting point, so
+  // the label's logit has been read)
+  sum = row_reduce<CS>(sum, false, smem32, &slot[1]);
+  if (threadIdx.x == 0 && rank == 0) row_loss[row] = -(at_label - top - log(sum));
+  if (GRAD) {
+    const double c = (gloss ? *gloss : 1.0) * inv_denom, scale = c / sum;
+#pragma unroll
+    for (int i = 0; i < kRowsValues / 4; i++) {
+      const int j = begin + (i * kRowsThreads + threadIdx.x) * 4;
+      if (j >= end) continue;
+      double q[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) q[k] = j + k == label ? fma(v[4 * i + k], scale, -c) : v[4 * i + k] * scale;
+      if (j + 3 < end) {
+        *reinterpret_cast<double4v *>(r + j) = double4v{q[0], q[1], q[2], q[3]};
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+          if (j + k < end) r[j + k] = q[k];
+      }
+    }
+  }
+  if (CS > 1) cooperative_groups::this_cluster().sync();  // nobody leaves while its slots may be read
+}
+
+// The same for rows that eight CTAs cannot hold (over 65 536 classes): the running
+// maximum and sum of each thread in one pass, p in a second.
+template <bool GRAD>
+__global__ void __launch_bounds__(kRowsThreads)
+xent_long_rows_kernel(double *__restrict__ z, const int *__restrict__ labels, const double *__restrict__ gloss,
+                      double *__restrict__ row_loss, int V, size_t pitch, double inv_denom, int *status) {
   __shared__ double smem32[32];
   double *r = z + (size_t)blockIdx.x * pitch;
   const int label = labels[blockIdx.x];
-  const bool keep = label >= 0 && (size_t)label < V;
+  const bool keep = label >= 0 && label < V;
   if (!keep) {
     if (threadIdx.x == 0) {
-      if (label != -1) atomicExch(status, 101);  // not a class and not "left out"
+      if (label != -1) atomicExch(status, 101);
       row_loss[blockIdx.x] = 0.0;
     }
     if (GRAD)
-      for (size_t j = threadIdx.x; j < pitch; j += kXentThreads) r[j] = 0.0;
+      for (int j = threadIdx.x; j < V; j += kRowsThreads) r[j] = 0.0;
     return;
   }
-  double top = -INFINITY;
-  for (size_t j = threadIdx.x; j < V; j += kXentThreads) top = fmax(top, r[j]);
-  top = block_reduce(top, true, smem32);
-  double sum = 0.0;
-  for (size_t j = threadIdx.x; j < V; j += kXentThreads) sum += exp(r[j] - top);
-  sum = block_reduce(sum, false, smem32);
+  double own = -INFINITY, sum = 0.0;
+  for (int j0 = threadIdx.x; j0 < V; j0 += 8 * kRowsThreads) {
+    double v[8], m = own;
+#pragma unroll
+    for (int k = 0; k < 8; k++) v[k] = j0 + k * kRowsThreads < V ? r[j0 + k * kRowsThreads] : -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 8; k++) m = fmax(m, v[k]);
+    if (m > own) {
+      sum *= exp(own - m);
+      own = m;
+    }
+    // (own stays -inf while all classes so far have probability 0; a NaN enters the sum)
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+      if (j0 + k * kRowsThreads < V) sum += v[k] == -INFINITY ? 0.0 : exp(v[k] - own);
+  }
+  const double top = block_reduce(own, true, smem32);
+  sum = block_reduce(own == -INFINITY && sum == 0.0 ? 0.0 : sum * exp(own - top), false, smem32);
   if (threadIdx.x == 0) row_loss[blockIdx.x] = -(r[label] - top - log(sum));
   if (GRAD) {
     __syncthreads();
-    const double scale = (gloss ? *gloss : 1.0) * inv_denom, unit = 1.0 / sum;
-    for (size_t j = threadIdx.x; j < pitch; j += kXentThreads)
-      r[j] = j < V ? scale * (exp(r[j] - top) * unit - (j == (size_t)label ? 1.0 : 0.0)) : 0.0;
+    const double c = (gloss ? *gloss : 1.0) * inv_denom, scale = c / sum;
+    for (int j0 = threadIdx.x; j0 < V; j0 += 8 * kRowsThreads) {
+      double v[8];
+#pragma unroll
+      for (int k = 0; k < 8; k++) v[k] = j0 + k * kRowsThreads < V ? r[j0 + k * kRowsThreads] : 0.0;
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        const int j = j0 + k * kRowsThreads;
+        if (j < V) r[j] = j == label ? fma(exp(v[k] - top), scale, -c) : exp(v[k] - top) * scale;
+      }
+    }
   }
+}
+
+template <bool GRAD, int CS>
+static int launch_rows(double *z, const int *labels, const double *gloss, double *row_loss, size_t rows, size_t V,
+                       size_t pitch, double inv_denom) {
+  Context &c = ctx();
+  const size_t piece = ((V + CS - 1) / CS + 3) / 4 * 4;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(rows * CS));
+  cfg.blockDim = dim3(kRowsThreads);
+  cfg.stream = c.stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CS;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CS > 1 ? 1 : 0;
+  MG_CUDA_TRY(cudaLaunchKernelEx(&cfg, xent_rows_kernel<GRAD, CS>, z, labels, gloss, row_loss, (int)V, pitch,
+                                 (int)piece, inv_denom, c.kernel_status));
+  MG_LAUNCH_CHECK("linear_xent rows");
+  return MG_OK;
+}
+
+template <bool GRAD>
+static int softmax_rows(double *z, const int *labels, const double *gloss, double *row_loss, size_t rows, size_t V,
+                        size_t pitch, double inv_denom) {
+  Context &c = ctx();
+  const size_t room = (size_t)kRowsThreads * kRowsValues;
+  if (V > 8 * room) {
+    xent_long_rows_kernel<GRAD><<<(unsigned)rows, kRowsThreads, 0, c.stream>>>(z, labels, gloss, row_loss, (int)V,
+                                                                             pitch, inv_denom, c.kernel_status);
+    MG_LAUNCH_CHECK("linear_xent rows");
+    return MG_OK;
+  }
+  // As few CTAs per row as hold it, more while that leaves SMs without any.
+  size_t cs = 1;
+  while (cs * (room - 4) < V && cs < 8) cs *= 2;
+  while (cs < 8 && rows * cs < (size_t)c.sm_count && V / cs > 2048) cs *= 2;
+  if (cs == 1) return launch_rows<GRAD, 1>(z, labels, gloss, row_loss, rows, V, pitch, inv_denom);
+  if (cs == 2) return launch_rows<GRAD, 2>(z, labels, gloss, row_loss, rows, V, pitch, inv_denom);
+  if (cs == 4) return launch_rows<GRAD, 4>(z, labels, gloss, row_loss, rows, V, pitch, inv_denom);
+  return launch_rows<GRAD, 8>(z, labels, gloss, row_loss, rows, V, pitch, inv_denom);
 }
 
 // loss[0] = sum of the rows' losses / denom, one CTA, fixed order.
@@ -179,13 +336,9 @@ static int run_head(const Head &h) {
       fwd.ldb = ldw;
       fwd.ldd = Vp;
       if ((r = run_gemm_ext(fwd)) != MG_OK) return r;
-      if (h.grad)
-        xent_rows_kernel<true><<<(unsigned)rows, kXentThreads, 0, c.stream>>>(
-            z, h.labels + m0, h.gloss, ws + at_loss + m0, h.V, Vp, inv, c.kernel_status);
-      else
-        xent_rows_kernel<false><<<(unsigned)rows, kXentThreads, 0, c.stream>>>(
-            z, h.labels + m0, h.gloss, ws + at_loss + m0, h.V, Vp, inv, c.kernel_status);
-      MG_LAUNCH_CHECK("linear_xent rows");
+      r = h.grad ? softmax_rows<true>(z, h.labels + m0, h.gloss, ws + at_loss + m0, rows, h.V, Vp, inv)
+                 : softmax_rows<false>(z, h.labels + m0, h.gloss, ws + at_loss + m0, rows, h.V, Vp, inv);
+      if (r != MG_OK) return r;
       const bool first = m0 == 0;
       if (h.grad && h.gx) {
         GemmExt e{{z, w, h.gx + m0 * h.K, rows, h.K, h.V, true, true, !(h.flags & MG_ACC_STORE_A), MG_EPI_NONE, nullptr}};

@@ -21,53 +21,168 @@ namespace mg {
 constexpr int kQ8Threads = 256;
 constexpr int kQ8Block = MG_Q8_BLOCK;
 constexpr double kQ8MaxScale = 0x1.0204081020407p+1017;  // largest s with 127 s finite
-static_assert(kQ8Block == 64, "the kernels deal a block to the lanes of a warp two columns each");
+static_assert(kQ8Block == 64, "the kernels deal a block to 16 or 32 lanes");
 
 __device__ __forceinline__ double q8_inverse(double top) { return top >= 1e-300 ? 127.0 / top : 0.0; }
 
+// rint(x * inverse), |x * inverse| < 128, as the low word of the sum with 1.5 * 2^52
+// (ties to even, like rint); the sign of x where that is 0 and x is not.
 __device__ __forceinline__ int q8_code(double x, double inverse) {
-  const int q = (int)rint(x * inverse);
-  return q != 0 ? q : (x > 0 ? 1 : (x < 0 ? -1 : 0));
+  const int q = __double2loint(x * inverse + 6755399441055744.0);
+  const int hi = __double2hiint(x), some = (hi << 1) | __double2loint(x);
+  return q != 0 || some == 0 ? q : (hi < 0 ? -1 : 1);
 }
 
-// A warp per block, lane l the columns l and l + 32.
-__global__ void __launch_bounds__(kQ8Threads)
-q8_pack_kernel(const double *__restrict__ x, signed char *__restrict__ codes, double *__restrict__ scales,
-               size_t M, size_t N, size_t nb) {
-  const int lane = threadIdx.x & 31;
-  const size_t warps = (size_t)gridDim.x * (kQ8Threads / 32), blocks = M * nb;
-  for (size_t b = (size_t)blockIdx.x * (kQ8Threads / 32) + (threadIdx.x >> 5); b < blocks; b += warps) {
-    const size_t row = b / nb, c0 = (b - row * nb) * kQ8Block, at = row * N + c0;
-    const bool in0 = c0 + lane < N, in1 = c0 + lane + 32 < N;
-    const double v0 = in0 ? x[at + lane] : 0.0, v1 = in1 ? x[at + lane + 32] : 0.0;
-    // NaN > infinity > every finite number in the order of the bit patterns of |x|.
-    unsigned long long m0 = __double_as_longlong(fabs(v0)), m1 = __double_as_longlong(fabs(v1));
-    unsigned long long m = m0 > m1 ? m0 : m1;
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-      const unsigned long long o = __shfl_xor_sync(0xffffffffu, m, off);
-      m = o > m ? o : m;
-    }
-    const double top = __longlong_as_double((long long)m);
-    const bool finite = m < 0x7ff0000000000000ull;
-    const double inverse = finite ? q8_inverse(top) : 0.0;
-    if (in0) codes[at + lane] = (signed char)q8_code(finite ? v0 : copysign(v0 == v0 ? 1.0 : 0.0, v0), inverse);
-    if (in1) codes[at + lane + 32] = (signed char)q8_code(finite ? v1 : copysign(v1 == v1 ? 1.0 : 0.0, v1), inverse);
-    if (lane == 0)
-      scales[b] = !finite ? __longlong_as_double(0x7ff8000000000000ll) : inverse > 0.0 ? fmin(top / 127.0, kQ8MaxScale) : 0.0;
+// Reads and writes of VEC neighbouring values and codes.
+template <int VEC> __device__ __forceinline__ void load_values(const double *p, double (&v)[VEC]) {
+  if constexpr (VEC == 4) {
+    const double4v t = ld_stream_v4(reinterpret_cast<const double4v *>(p));
+    v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+  } else if constexpr (VEC == 2) {
+    const double2 t = __ldcs(reinterpret_cast<const double2 *>(p));
+    v[0] = t.x; v[1] = t.y;
+  } else {
+    v[0] = __ldcs(p);
   }
 }
 
+// LANES lanes take a block, VEC neighbouring columns each, UN blocks at a time so that
+// 64 to 128 bytes per lane are on their way.  A lane of a block's ragged end has no
+// column; LANES x VEC = 64.
+template <int VEC, int UN, bool FLAT>
+__global__ void __launch_bounds__(kQ8Threads)
+q8_pack_kernel(const double *__restrict__ x, signed char *__restrict__ codes, double *__restrict__ scales,
+               size_t blocks, size_t N, unsigned nb) {
+  constexpr int LANES = VEC == 4 ? 16 : 32, PER = 64 / LANES;  // columns per lane
+  const int lane = threadIdx.x % LANES;
+  const size_t teams = (size_t)gridDim.x * (kQ8Threads / LANES);
+  // (all lanes of a warp make the same number of rounds: they shuffle together)
+  const size_t first = ((size_t)blockIdx.x * kQ8Threads + threadIdx.x) / LANES, rounds = (blocks + teams * UN - 1) / (teams * UN);
+  for (size_t round = 0; round < rounds; round++) {
+    double v[UN][PER];
+    size_t at[UN];
+    int cols[UN];  // columns of this lane
+#pragma unroll
+    for (int u = 0; u < UN; u++) {
+      const size_t b = first + (round * UN + u) * teams;
+      cols[u] = 0;
+      if (b < blocks) {
+        if (FLAT) {
+          at[u] = b * 64 + lane * PER;
+          cols[u] = PER;
+        } else {
+          const size_t row = blocks >> 32 ? b / nb : (size_t)((unsigned)b / nb);
+          const size_t c = (b - row * nb) * 64 + lane * PER;
+          at[u] = row * N + c;
+          cols[u] = c < N ? (N - c < PER ? (int)(N - c) : PER) : 0;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < PER; k++) v[u][k] = 0.0;
+      if constexpr (VEC == PER) {
+        if (cols[u] > 0) load_values<VEC>(x + at[u], v[u]);  // (N is a multiple of VEC)
+      } else {
+#pragma unroll
+        for (int k = 0; k < PER; k++)
+          if (k < cols[u]) v[u][k] = __ldcs(x + at[u] + k);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < UN; u++) {
+      // NaN > infinity > every finite number in the order of the bit patterns of |x|.
+      unsigned long long m = 0;
+#pragma unroll
+      for (int k = 0; k < PER; k++) {
+        const unsigned long long o = (unsigned long long)__double_as_longlong(fabs(v[u][k]));
+        m = o > m ? o : m;
+      }
+#pragma unroll
+      for (int off = LANES / 2; off > 0; off >>= 1) {
+        const unsigned long long o = __shfl_xor_sync(0xffffffffu, m, off);
+        m = o > m ? o : m;
+      }
+      const double top = __longlong_as_double((long long)m);
+      const bool finite = m < 0x7ff0000000000000ull;
+      const double inverse = finite ? q8_inverse(top) : 0.0;
+      unsigned word = 0;
+#pragma unroll
+      for (int k = 0; k < PER; k++) {
+        double y = v[u][k];
+        if (!finite) y = y > 0 ? 1.0 : (y < 0 ? -1.0 : 0.0);
+        word |= (unsigned)(q8_code(y, inverse) & 255) << (8 * k);
+      }
+      if (VEC == PER && cols[u] > 0) {
+        if (PER == 4) *reinterpret_cast<unsigned *>(codes + at[u]) = word;
+        else *reinterpret_cast<unsigned short *>(codes + at[u]) = (unsigned short)word;
+      } else {
+#pragma unroll
+        for (int k = 0; k < PER; k++)
+          if (k < cols[u]) codes[at[u] + k] = (signed char)(word >> (8 * k));
+      }
+      const size_t b = first + (round * UN + u) * teams;
+      if (lane == 0 && b < blocks)
+        scales[b] = !finite ? __longlong_as_double(0x7ff8000000000000ll)
+                            : inverse > 0.0 ? fmin(top / 127.0, kQ8MaxScale) : 0.0;
+    }
+  }
+}
+
+template <int VEC, int UN, bool FLAT>
 __global__ void __launch_bounds__(kQ8Threads)
 q8_unpack_kernel(const signed char *__restrict__ codes, const double *__restrict__ scales,
-                 double *__restrict__ x, size_t M, size_t N, size_t nb) {
-  const int lane = threadIdx.x & 31;
-  const size_t warps = (size_t)gridDim.x * (kQ8Threads / 32), blocks = M * nb;
-  for (size_t b = (size_t)blockIdx.x * (kQ8Threads / 32) + (threadIdx.x >> 5); b < blocks; b += warps) {
-    const size_t row = b / nb, c0 = (b - row * nb) * kQ8Block, at = row * N + c0;
-    const double scale = scales[b];
-    if (c0 + lane < N) x[at + lane] = (double)codes[at + lane] * scale;
-    if (c0 + lane + 32 < N) x[at + lane + 32] = (double)codes[at + lane + 32] * scale;
+                 double *__restrict__ x, size_t blocks, size_t N, unsigned nb) {
+  constexpr int LANES = VEC == 4 ? 16 : 32, PER = 64 / LANES;
+  const int lane = threadIdx.x % LANES;
+  const size_t teams = (size_t)gridDim.x * (kQ8Threads / LANES);
+  for (size_t b0 = ((size_t)blockIdx.x * kQ8Threads + threadIdx.x) / LANES; b0 < blocks; b0 += teams * UN) {
+    unsigned word[UN];
+    double scale[UN];
+    size_t at[UN];
+    int cols[UN];
+#pragma unroll
+    for (int u = 0; u < UN; u++) {
+      const size_t b = b0 + u * teams;
+      cols[u] = 0;
+      word[u] = 0;
+      if (b < blocks) {
+        if (FLAT) {
+          at[u] = b * 64 + lane * PER;
+          cols[u] = PER;
+        } else {
+          const size_t row = blocks >> 32 ? b / nb : (size_t)((unsigned)b / nb);
+          const size_t c = (b - row * nb) * 64 + lane * PER;
+          at[u] = row * N + c;
+          cols[u] = c < N ? (N - c < PER ? (int)(N - c) : PER) : 0;
+        }
+      }
+      if (cols[u] > 0) {
+        scale[u] = __ldg(scales + b);
+        if constexpr (VEC == PER) {
+          if (PER == 4) word[u] = __ldcs(reinterpret_cast<const unsigned *>(codes + at[u]));
+          else word[u] = __ldcs(reinterpret_cast<const unsigned short *>(codes + at[u]));
+        } else {
+#pragma unroll
+          for (int k = 0; k < PER; k++)
+            if (k < cols[u]) word[u] |= (unsigned)(unsigned char)codes[at[u] + k] << (8 * k);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < UN; u++) {
+      if (cols[u] <= 0) continue;
+      double v[PER];
+#pragma unroll
+      for (int k = 0; k < PER; k++) v[k] = (double)(signed char)(word[u] >> (8 * k)) * scale[u];
+      if constexpr (VEC == PER && PER == 4) {
+        st_stream_v4(reinterpret_cast<double4v *>(x + at[u]), double4v{v[0], v[1], v[2], v[3]});
+      } else if constexpr (VEC == PER) {
+        __stcs(reinterpret_cast<double2 *>(x + at[u]), make_double2(v[0], v[1]));
+      } else {
+#pragma unroll
+        for (int k = 0; k < PER; k++)
+          if (k < cols[u]) x[at[u] + k] = v[k];
+      }
+    }
   }
 }
 
@@ -83,10 +198,18 @@ q8_relu_bwd_kernel(const signed char *__restrict__ codes, const double *g, doubl
   }
 }
 
+// Widest access that the row length and both addresses allow.
+static int q8_vec(const double *x, const signed char *codes, size_t N) {
+  const uintptr_t px = reinterpret_cast<uintptr_t>(x), pc = reinterpret_cast<uintptr_t>(codes);
+  if (N % 4 == 0 && px % 32 == 0 && pc % 4 == 0) return 4;
+  if (N % 2 == 0 && px % 16 == 0 && pc % 2 == 0) return 2;
+  return 1;
+}
+
 static size_t q8_blocks(size_t N) { return (N + kQ8Block - 1) / kQ8Block; }
 
 static int check_q8(const char *name, size_t M, size_t N) {
-  if (M >= ((size_t)1 << 40) || N >= ((size_t)1 << 40) || (M && N > ((size_t)1 << 60) / M))
+  if (M >= ((size_t)1 << 40) || N >= ((size_t)1 << 36) || (M && N > ((size_t)1 << 60) / M))
     return fail(MG_ERR_INVALID, "%s: dimension too large", name);
   return MG_OK;
 }
@@ -103,8 +226,18 @@ int mg_q8_pack(const double *x, signed char *codes, double *scales, size_t M, si
   if (M && N && (!x || !codes || !scales)) return fail(MG_ERR_INVALID, "mg_q8_pack: null pointer");
   MG_ENSURE_INIT();
   if (M == 0 || N == 0) return MG_OK;
-  const size_t nb = q8_blocks(N);
-  q8_pack_kernel<<<grid_for(M * nb * 32, kQ8Threads, 64), kQ8Threads, 0, ctx().stream>>>(x, codes, scales, M, N, nb);
+  const size_t nb = q8_blocks(N), blocks = M * nb;
+  cudaStream_t stream = ctx().stream;
+  const int vec = q8_vec(x, codes, N);
+  const unsigned grid = grid_for(blocks * (vec == 4 ? 16 : 32), kQ8Threads, 64);
+  if (vec == 4 && N % 64 == 0)
+    q8_pack_kernel<4, 4, true><<<grid, kQ8Threads, 0, stream>>>(x, codes, scales, blocks, N, (unsigned)nb);
+  else if (vec == 4)
+    q8_pack_kernel<4, 2, false><<<grid, kQ8Threads, 0, stream>>>(x, codes, scales, blocks, N, (unsigned)nb);
+  else if (vec == 2)
+    q8_pack_kernel<2, 4, false><<<grid, kQ8Threads, 0, stream>>>(x, codes, scales, blocks, N, (unsigned)nb);
+  else
+    q8_pack_kernel<1, 4, false><<<grid, kQ8Threads, 0, stream>>>(x, codes, scales, blocks, N, (unsigned)nb);
   MG_LAUNCH_CHECK("q8_pack");
   return MG_OK;
 }
@@ -115,8 +248,18 @@ int mg_q8_unpack(const signed char *codes, const double *scales, double *x, size
   if (M && N && (!x || !codes || !scales)) return fail(MG_ERR_INVALID, "mg_q8_unpack: null pointer");
   MG_ENSURE_INIT();
   if (M == 0 || N == 0) return MG_OK;
-  const size_t nb = q8_blocks(N);
-  q8_unpack_kernel<<<grid_for(M * nb * 32, kQ8Threads, 64), kQ8Threads, 0, ctx().stream>>>(codes, scales, x, M, N, nb);
+  const size_t nb = q8_blocks(N), blocks = M * nb;
+  cudaStream_t stream = ctx().stream;
+  const int vec = q8_vec(x, codes, N);
+  const unsigned grid = grid_for(blocks * (vec == 4 ? 16 : 32), kQ8Threads, 64);
+  if (vec == 4 && N % 64 == 0)
+    q8_unpack_kernel<4, 4, true><<<grid, kQ8Threads, 0, stream>>>(codes, scales, x, blocks, N, (unsigned)nb);
+  else if (vec == 4)
+    q8_unpack_kernel<4, 2, false><<<grid, kQ8Threads, 0, stream>>>(codes, scales, x, blocks, N, (unsigned)nb);
+  else if (vec == 2)
+    q8_unpack_kernel<2, 4, false><<<grid, kQ8Threads, 0, stream>>>(codes, scales, x, blocks, N, (unsigned)nb);
+  else
+    q8_unpack_kernel<1, 4, false><<<grid, kQ8Threads, 0, stream>>>(codes, scales, x, blocks, N, (unsigned)nb);
   MG_LAUNCH_CHECK("q8_unpack");
   return MG_OK;
 }
