@@ -28,7 +28,8 @@ struct GemmExt {
   GemmDesc d;
   size_t lda = 0, ldb = 0, ldd = 0;
   const signed char *mask8 = nullptr;   // [M][N]: output * (mask8 > 0)
-  const signed char *codes = nullptr;   // A = codes * scales, [K][M] (then d.A is null)
+  // A = codes * scales, [K][M], then d.A is null; row pitch lda and base multiples of 16
+  const signed char *codes = nullptr;
   const double *scales = nullptr;
 };
 int run_gemm_ext(const GemmExt &e);

@@ -103,6 +103,8 @@ int run_gemm_ext(const GemmExt &e) {
     return MG_OK;
   }
   if (!q8 && !e.mask8 && dense && (d.M > 64 || d.N <= (size_t)SkinnyCfg::BN)) return run_gemm(d);
+  if (q8 && (lda % 16 != 0 || off_16_bytes(e.codes)))
+    return fail(MG_ERR_INVALID, "gemm: rows of codes do not start on 16-byte boundaries");
   if ((!q8 && ((lda & 1) || off_16_bytes(d.A))) || (ldb & 1) || off_16_bytes(d.B))
     return fail(MG_ERR_INVALID, "gemm: operand rows do not start on 16-byte boundaries");
   Context &c = ctx();
@@ -116,7 +118,6 @@ int run_gemm_ext(const GemmExt &e) {
     L.qa.ldc = lda;
     L.qa.blocks = (d.M + MG_Q8_BLOCK - 1) / MG_Q8_BLOCK;
     L.qa.cols = M;
-    L.qa.wide = lda % 16 == 0 && !off_16_bytes(e.codes);
   } else if (d.a_kcontig) {
     ok_a = make_tensor_map_f64(&L.ma, d.A, d.M, d.K, BK, plan.bm, lda);
   } else if (lda % 16 == 0 && make_tensor_map_f64_grouped(&L.ma, d.A, d.K, lda, BK, plan.bm / 16)) {

@@ -208,6 +208,149 @@ static int q8_vec(const double *x, const signed char *codes, size_t N) {
 
 static size_t q8_blocks(size_t N) { return (N + kQ8Block - 1) / kQ8Block; }
 
+// dst[rows][pitch] = src[rows][cols], zeros behind them (pitch a multiple of 16).
+__global__ void __launch_bounds__(256)
+q8_copy_rows_kernel(const signed char *__restrict__ src, size_t rows, size_t cols, signed char *__restrict__ dst,
+                    size_t pitch) {
+  const size_t words = pitch / 4, all = rows * words;
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (size_t)gridDim.x * 256) {
+    const size_t r = all >> 32 ? i / words : (size_t)((unsigned)i / (unsigned)words), c = (i - r * words) * 4;
+    const signed char *p = src + r * cols + c;
+    unsigned w = 0;
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+      if (c + k < cols) w |= (unsigned)(unsigned char)p[k] << (8 * k);
+    reinterpret_cast<unsigned *>(dst)[i] = w;
+  }
+}
+
+static int copy_codes_rows(const signed char *src, size_t rows, size_t cols, signed char *dst, size_t pitch) {
+  q8_copy_rows_kernel<<<grid_for(rows * pitch / 4, 256, 32), 256, 0, ctx().stream>>>(src, rows, cols, dst, pitch);
+  MG_LAUNCH_CHECK("copy of codes");
+  return MG_OK;
+}
+
+// dA[M][K] (+)= (G[M][N] . B[K][N]^T) * (mask > 0) for N <= 16: nothing but streaming
+// the output, 9 bytes per element (17 when accumulating) against 2 N flop.  A thread
+// keeps two columns' rows of B in registers and walks down the rows; the rows of G pass
+// through shared memory, where a warp reads each value once for its 64 outputs.
+// PAIR: the two columns are neighbours (K even, aligned), else TX apart.  The next
+// rows of G and of the mask are on their way while a block of rows is computed.
+constexpr int kOuterRows = 8;  // rows per thread and block
+
+template <int NN, bool PAIR>
+__global__ void __launch_bounds__(256, 2)
+q8_outer_kernel(const double *__restrict__ G, const double *__restrict__ B, double *dA,
+                const signed char *__restrict__ mask, size_t M, int N, size_t K, bool accumulate) {
+  constexpr int kMostTY = 8, kPer = (kOuterRows * kMostTY * NN + 255) / 256;
+  __shared__ __align__(16) double gs[2][kOuterRows * kMostTY * NN];
+  const int TX = blockDim.x, TY = blockDim.y, tid = threadIdx.y * TX + threadIdx.x;
+  const size_t c0 = (size_t)blockIdx.x * 2 * TX + (PAIR ? 2 * threadIdx.x : threadIdx.x), c1 = PAIR ? c0 + 1 : c0 + TX;
+  const bool in0 = c0 < K, in1 = c1 < K;
+  double b0[NN], b1[NN];
+#pragma unroll
+  for (int n = 0; n < NN; n++) {
+    b0[n] = in0 && n < N ? B[c0 * N + n] : 0.0;
+    b1[n] = in1 && n < N ? B[c1 * N + n] : 0.0;
+  }
+  const int rows = kOuterRows * TY, values = rows * NN;
+  const size_t blocks = (M + rows - 1) / rows;
+  unsigned short next[kOuterRows];  // a row's two codes
+  double g_next[kPer];
+  auto read = [&](size_t blk) {
+    const size_t m0 = blk * rows;
+#pragma unroll
+    for (int u = 0; u < kOuterRows; u++) {
+      const size_t m = m0 + u * TY + threadIdx.y, at = m * K;
+      next[u] = 0;
+      if (m < M) {
+        if (PAIR) {
+          if (in0) next[u] = __ldcs(reinterpret_cast<const unsigned short *>(mask + at + c0));
+        } else {
+          if (in0) next[u] = (unsigned char)mask[at + c0];
+          if (in1) next[u] |= (unsigned short)((unsigned char)mask[at + c1] << 8);
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kPer; k++) {
+      const int i = tid + 256 * k, r = i / NN, n = i % NN;
+      g_next[k] = i < values && m0 + r < M && n < N ? __ldg(G + (m0 + r) * N + n) : 0.0;
+    }
+  };
+  auto hand_over = [&](int buf) {
+#pragma unroll
+    for (int k = 0; k < kPer; k++)
+      if (tid + 256 * k < values) gs[buf][tid + 256 * k] = g_next[k];
+  };
+  size_t blk = blockIdx.y;
+  if (blk < blocks) read(blk);
+  hand_over(0);
+  int buf = 0;
+  for (; blk < blocks; blk += gridDim.y, buf ^= 1) {
+    __syncthreads();  // gs[buf] is complete, and nobody reads the other one any more
+    unsigned short codes[kOuterRows];
+#pragma unroll
+    for (int u = 0; u < kOuterRows; u++) codes[u] = next[u];
+    if (blk + gridDim.y < blocks) read(blk + gridDim.y);
+#pragma unroll
+    for (int u = 0; u < kOuterRows; u++) {
+      const int r = u * TY + threadIdx.y;
+      const size_t m = blk * rows + r;
+      if (m >= M) continue;
+      const double *g = &gs[buf][r * NN];
+      double s0 = 0.0, s1 = 0.0;
+#pragma unroll
+      for (int n = 0; n < NN; n += 2) {
+        const double2 v = *reinterpret_cast<const double2 *>(g + n);
+        s0 = fma(v.x, b0[n], s0);
+        s1 = fma(v.x, b1[n], s1);
+        s0 = fma(v.y, b0[n + 1], s0);
+        s1 = fma(v.y, b1[n + 1], s1);
+      }
+      s0 = s0 * ((signed char)codes[u] > 0 ? 1.0 : 0.0);
+      s1 = s1 * ((short)codes[u] >= 256 ? 1.0 : 0.0);  // (its high byte > 0)
+      double *dst = dA + m * K;
+      if (PAIR) {
+        if (!in0) continue;
+        if (accumulate) {
+          const double2 o = *reinterpret_cast<const double2 *>(dst + c0);
+          s0 = o.x + s0;
+          s1 = o.y + s1;
+        }
+        __stcs(reinterpret_cast<double2 *>(dst + c0), make_double2(s0, s1));
+      } else {
+        if (in0) dst[c0] = accumulate ? dst[c0] + s0 : s0;
+        if (in1) dst[c1] = accumulate ? dst[c1] + s1 : s1;
+      }
+    }
+    hand_over(buf ^ 1);
+  }
+}
+
+static int outer_q8(const double *G, const double *B, double *dA, size_t M, size_t N, size_t K, int accumulate,
+                    const signed char *mask) {
+  unsigned tx = 32;
+  while (tx < 256 && 2 * (size_t)tx < K) tx *= 2;
+  const bool pair = K % 2 == 0 && !off_16_bytes(dA) && !(reinterpret_cast<uintptr_t>(mask) & 1);
+  const size_t rows = (size_t)kOuterRows * (256 / tx), gx = (K + 2 * tx - 1) / (2 * tx), blocks = (M + rows - 1) / rows;
+  size_t gy = (size_t)ctx().sm_count * 16 / gx + 1;
+  if (gy > blocks) gy = blocks;
+  if (gy > 65535) gy = 65535;
+  const dim3 grid((unsigned)gx, (unsigned)gy), block(tx, 256 / tx);
+  cudaStream_t stream = ctx().stream;
+#define MG_OUTER(NN)                                                                                        \
+  (pair ? q8_outer_kernel<NN, true><<<grid, block, 0, stream>>>(G, B, dA, mask, M, (int)N, K, accumulate != 0) \
+        : q8_outer_kernel<NN, false><<<grid, block, 0, stream>>>(G, B, dA, mask, M, (int)N, K, accumulate != 0))
+  if (N <= 4) MG_OUTER(4);
+  else if (N <= 8) MG_OUTER(8);
+  else if (N <= 12) MG_OUTER(12);
+  else MG_OUTER(16);
+#undef MG_OUTER
+  MG_LAUNCH_CHECK("gemm_nt_q8 (few columns)");
+  return MG_OK;
+}
+
 static int check_q8(const char *name, size_t M, size_t N) {
   if (M >= ((size_t)1 << 40) || N >= ((size_t)1 << 36) || (M && N > ((size_t)1 << 60) / M))
     return fail(MG_ERR_INVALID, "%s: dimension too large", name);
@@ -283,19 +426,31 @@ int mg_gemm_tn_q8(const signed char *codes, const double *scales, const double *
   MG_ENSURE_INIT();
   if (K == 0 || N == 0) return MG_OK;
   // Output [K][N], contraction over the M rows; the codes are widened inside the kernel.
+  // Rows of codes or of G that it cannot take are copied into rows that it can.
   GemmExt e{{nullptr, G, dB, K, N, M, false, false, accumulate, MG_EPI_NONE, nullptr}};
   e.codes = codes;
   e.scales = scales;
-  if (N % 2 == 0 && !off_16_bytes(G)) return run_gemm_ext(e);
-  // Rows of G that the tensor kernel cannot take are copied into rows it can.
-  double *g = nullptr;
-  e.ldb = pitch16(N);
-  rc = mg_alloc(M * e.ldb, &g);
+  e.lda = K;
+  const bool copy_codes = K % 16 != 0 || off_16_bytes(codes), copy_g = N % 2 != 0 || off_16_bytes(G);
+  if (!copy_codes && !copy_g) return run_gemm_ext(e);
+  const size_t pitch_c = pitch16(K), pitch_g = pitch16(N);
+  const size_t code_room = copy_codes ? (M * pitch_c + 255) / 256 * 32 : 0;  // in doubles
+  double *room = nullptr;
+  rc = mg_alloc(code_room + (copy_g ? M * pitch_g : 0), &room);
   if (rc != MG_OK) return rc;
-  rc = copy_rows(G, M, N, N, g, e.ldb);
-  e.d.B = g;
+  if (copy_codes) {
+    signed char *dst = reinterpret_cast<signed char *>(room);
+    rc = copy_codes_rows(codes, M, K, dst, pitch_c);
+    e.codes = dst;
+    e.lda = pitch_c;
+  }
+  if (rc == MG_OK && copy_g) {
+    rc = copy_rows(G, M, N, N, room + code_room, pitch_g);
+    e.d.B = room + code_room;
+    e.ldb = pitch_g;
+  }
   if (rc == MG_OK) rc = run_gemm_ext(e);
-  const int freed = mg_free(g);
+  const int freed = mg_free(room);
   return rc != MG_OK ? rc : freed;
 }
 
@@ -305,6 +460,7 @@ int mg_gemm_nt_q8(const double *G, const double *B, double *dA, size_t M, size_t
     return fail(MG_ERR_INVALID, "mg_gemm_nt_q8: null pointer");
   MG_ENSURE_INIT();
   if (M == 0 || K == 0) return MG_OK;
+  if (N > 0 && N <= 16) return outer_q8(G, B, dA, M, N, K, accumulate, mask_codes);
   // Output [M][K], contraction over N.
   GemmExt e{{G, B, dA, M, K, N, true, true, accumulate, MG_EPI_NONE, nullptr}};
   e.mask8 = mask_codes;
