@@ -284,8 +284,8 @@ int mg_q8_pack(const double *x, signed char *codes, double *scales, size_t M, si
 int mg_q8_unpack(const signed char *codes, const double *scales, double *x, size_t M, size_t N);
 /* The backward pass on the 8-bit form.  mg_gemm_tn and mg_gemm_nt with
  * MG_EPI_RELU_MASK, their A operand / mask source in 8 bits:
- *   dB[K,N] (+)= x[M,K]^T . G[M,N],  x = the values codes and scales keep (computed as
- *                codes^T . (scale G): scale times an element of G must not overflow);
+ *   dB[K,N] (+)= x[M,K]^T . G[M,N],  x = the values codes and scales keep (in pieces of
+ *                rows, in a workspace of at most 256 MiB or 64 rows, where N > 32);
  *   dA[M,K] (+)= (G[M,N] . B[K,N]^T) * (mask_codes[M,K] > 0);
  * and the ReLU mask alone: gx[n] += g[n] * (codes[n] > 0). */
 int mg_gemm_tn_q8(const signed char *codes, const double *scales, const double *G, double *dB,

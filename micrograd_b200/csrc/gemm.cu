@@ -285,6 +285,7 @@ void gemm_release_tables() {
   for (auto &t : g_seg_tables) {
     cudaFree(t.dev_items);
     cudaFree(t.dev_tickets);
+    cudaFree(t.dev_tiles);
   }
   g_seg_tables.clear();
 }
@@ -376,6 +377,8 @@ int seg_table_for(int tiles_m, int tiles_n, int KT, int bm, int bn, int spans,
   t.min_nkt = min_nkt;
   MG_CUDA_TRY(cudaMalloc(&t.dev_items, segs.size() * sizeof(SegItem)));
   MG_CUDA_TRY(cudaMalloc(&t.dev_tickets, tile_info.size() * sizeof(unsigned int)));
+  MG_CUDA_TRY(cudaMalloc(&t.dev_tiles, tile_info.size() * sizeof(int2)));
+  MG_CUDA_TRY(cudaMemcpy(t.dev_tiles, tile_info.data(), tile_info.size() * sizeof(int2), cudaMemcpyHostToDevice));
   MG_CUDA_TRY(cudaMemset(t.dev_tickets, 0, tile_info.size() * sizeof(unsigned int)));
   MG_CUDA_TRY(cudaMemcpy(t.dev_items, segs.data(), segs.size() * sizeof(SegItem),
                          cudaMemcpyHostToDevice));

@@ -19,18 +19,15 @@ struct GemmDesc {
 int run_gemm(const GemmDesc &d);
 
 // The same on the tensor-core kernel with what the dense form does not know: row
-// pitches (0: dense), any row lengths of the output, few rows, an output mask or the A
-// operand of a transposed-A product in 8 bits.  A and B (or the codes) may have any
-// extents, but fp64 operands need even row pitches and 16-byte aligned bases, and an
-// operand whose contiguous axis is not k must have memory up to a pitch that is a
-// multiple of 16 where its row length is none (what it holds there is not used).
+// pitches (0: dense), any row lengths of the output, few rows, or an output mask in 8
+// bits.  A and B may have any extents, but need even row pitches and 16-byte aligned
+// bases, and an operand whose contiguous axis is not k must have memory up to a pitch
+// that is a multiple of 16 where its row length is none (what it holds there is not
+// used).
 struct GemmExt {
   GemmDesc d;
   size_t lda = 0, ldb = 0, ldd = 0;
-  const signed char *mask8 = nullptr;   // [M][N]: output * (mask8 > 0)
-  // A = codes * scales, [K][M], then d.A is null; row pitch lda and base multiples of 16
-  const signed char *codes = nullptr;
-  const double *scales = nullptr;
+  const signed char *mask8 = nullptr;  // [M][N]: output * (mask8 > 0)
 };
 int run_gemm_ext(const GemmExt &e);
 

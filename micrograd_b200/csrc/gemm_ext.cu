@@ -6,43 +6,59 @@ namespace mg {
 
 // One instantiation per tile, contraction split and grid form; all can skip the
 // ragged border (EDGE) and write any output (ANYD).
-template <bool AK, bool BK_, class Cfg, bool Q8A> static int launch_ext(const DmmaLaunch &L) {
-  if (L.tickets) return launch_dmma_masked<AK, BK_, 2, true, Cfg, false, false, true, true, Q8A>(L);
+template <bool AK, bool BK_, class Cfg> static int launch_ext(const DmmaLaunch &L) {
+  if (L.tickets) return launch_dmma_masked<AK, BK_, 2, true, Cfg, false, false, true, true>(L);
   if (!L.table && (L.min_nkt < 32 || Cfg::BN <= 32) && L.items > ctx().sm_count)
-    return launch_dmma_masked<AK, BK_, 2, true, Cfg, true, false, false, true, Q8A>(L);
-  return launch_dmma_masked<AK, BK_, 2, true, Cfg, false, false, false, true, Q8A>(L);
+    return launch_dmma_masked<AK, BK_, 2, true, Cfg, true, false, false, true>(L);
+  return launch_dmma_masked<AK, BK_, 2, true, Cfg, false, false, false, true>(L);
 }
 
 template <bool AK, bool BK_> static int launch_layout_ext(int tile, const DmmaLaunch &L) {
   switch (tile) {
-    case kTileSkinny: return launch_ext<AK, BK_, SkinnyCfg, false>(L);
-    case kTileSkinny16: return launch_ext<AK, BK_, Skinny16Cfg, false>(L);
-    case kTileHalf: return launch_ext<AK, BK_, HalfCfg, false>(L);
-    case kTileRows16: return launch_ext<AK, BK_, Rows16Cfg, false>(L);
-    case kTileRows32: return launch_ext<AK, BK_, Rows32Cfg, false>(L);
-    case kTileRows64: return launch_ext<AK, BK_, Rows64Cfg, false>(L);
-    default: return launch_ext<AK, BK_, MainCfg, false>(L);
-  }
-}
-
-static int launch_q8(int tile, const DmmaLaunch &L) {
-  switch (tile) {
-    case kTileSkinny: return launch_ext<false, false, SkinnyCfg, true>(L);
-    case kTileSkinny16: return launch_ext<false, false, Skinny16Cfg, true>(L);
-    case kTileHalf: return launch_ext<false, false, HalfCfg, true>(L);
-    default: return launch_ext<false, false, MainCfg, true>(L);
+    case kTileSkinny: return launch_ext<AK, BK_, SkinnyCfg>(L);
+    case kTileSkinny16: return launch_ext<AK, BK_, Skinny16Cfg>(L);
+    case kTileHalf: return launch_ext<AK, BK_, HalfCfg>(L);
+    case kTileRows16: return launch_ext<AK, BK_, Rows16Cfg>(L);
+    case kTileRows32: return launch_ext<AK, BK_, Rows32Cfg>(L);
+    case kTileRows64: return launch_ext<AK, BK_, Rows64Cfg>(L);
+    default: return launch_ext<AK, BK_, MainCfg>(L);
   }
 }
 
 // Few rows go to tiles of few rows, unless the columns are few as well.
-static GemmPlan plan_ext(int M, int N, int K, int sms, bool q8) {
-  if (!q8 && M <= 64 && N > SkinnyCfg::BN) {
+static GemmPlan plan_ext(int M, int N, int K, int sms) {
+  if (M <= 64 && N > SkinnyCfg::BN) {
     GemmPlan p = M <= 16 ? GemmPlan{kTileRows16, 16, 128, 0}
                          : (M <= 32 ? GemmPlan{kTileRows32, 32, 128, 0} : GemmPlan{kTileRows64, 64, 128, 0});
     p.spans = choose_spans((N + 127) / 128, (K + BK - 1) / BK, sms);
     return p;
   }
   return choose_plan(M, N, K, sms, 2, false);
+}
+
+// Adds up the partial tiles of split tiles, in slot (= k) order, a thread per output
+// element, and runs the epilogue.  The kernel's own fold has one CTA per tile, which is
+// right for many tiles; for few it is the longest part: 148 partial tiles of 128 x 64
+// take one CTA over 100 us and all SMs 4.
+constexpr int kFoldBySegments = 6;  // fold here from this many segments per tile on
+
+__global__ void __launch_bounds__(256)
+fold_tiles_kernel(GemmEpilogue ep, const int2 *__restrict__ tiles, int tiles_n, int bm, int bn, int M, int N) {
+  const int2 info = tiles[blockIdx.y];
+  if (info.y == 0) return;  // a whole tile: written by the kernel itself
+  const int e = blockIdx.x * 256 + threadIdx.x, r = e / bn, c = e - r * bn;
+  const int row = (blockIdx.y / tiles_n) * bm + r, col = (blockIdx.y % tiles_n) * bn + c;
+  if (r >= bm || row >= M || col >= N) return;
+  const size_t slot = (size_t)bm * bn;
+  const double *part = ep.partial + info.x * slot + e;
+  double v = 0.0;
+#pragma unroll 8
+  for (int k = 0; k < info.y; k++) v += __ldcs(part + k * slot);
+  if (ep.mode == MG_EPI_BIAS || ep.mode == MG_EPI_BIAS_RELU) v += __ldg(ep.aux + col);
+  if (ep.mode == MG_EPI_BIAS_RELU) v = v > 0 ? v : 0.0;
+  if (ep.mask8) v = v * (ep.mask8[(size_t)row * ep.ld_mask8 + col] > 0 ? 1.0 : 0.0);
+  double *dst = ep.D + (size_t)row * ep.ldd + col;
+  *dst = ep.accumulate ? *dst + v : v;
 }
 
 __global__ void __launch_bounds__(256)
@@ -86,7 +102,6 @@ empty_product_kernel(double *D, size_t M, size_t N, size_t ldd, int mode, const 
 
 int run_gemm_ext(const GemmExt &e) {
   const GemmDesc &d = e.d;
-  const bool q8 = e.codes != nullptr;
   if (d.M == 0 || d.N == 0) return MG_OK;
   const size_t lim = (size_t)1 << 30;
   if (d.M >= lim || d.N >= lim || d.K >= lim) return fail(MG_ERR_INVALID, "gemm: dimension too large");
@@ -102,25 +117,18 @@ int run_gemm_ext(const GemmExt &e) {
     MG_LAUNCH_CHECK("gemm (empty contraction)");
     return MG_OK;
   }
-  if (!q8 && !e.mask8 && dense && (d.M > 64 || d.N <= (size_t)SkinnyCfg::BN)) return run_gemm(d);
-  if (q8 && (lda % 16 != 0 || off_16_bytes(e.codes)))
-    return fail(MG_ERR_INVALID, "gemm: rows of codes do not start on 16-byte boundaries");
-  if ((!q8 && ((lda & 1) || off_16_bytes(d.A))) || (ldb & 1) || off_16_bytes(d.B))
+  if (!e.mask8 && dense && (d.M > 64 || d.N <= (size_t)SkinnyCfg::BN)) return run_gemm(d);
+  if ((lda & 1) || off_16_bytes(d.A) || (ldb & 1) || off_16_bytes(d.B))
     return fail(MG_ERR_INVALID, "gemm: operand rows do not start on 16-byte boundaries");
   Context &c = ctx();
   const int M = (int)d.M, N = (int)d.N, K = (int)d.K;
-  const GemmPlan plan = plan_ext(M, N, K, c.sm_count, q8);
+  const GemmPlan plan = plan_ext(M, N, K, c.sm_count);
   DmmaLaunch L{};
-  bool ok_a = true, ok_b;
-  if (q8) {
-    L.qa.codes = e.codes;
-    L.qa.scales = e.scales;
-    L.qa.ldc = lda;
-    L.qa.blocks = (d.M + MG_Q8_BLOCK - 1) / MG_Q8_BLOCK;
-    L.qa.cols = M;
-  } else if (d.a_kcontig) {
+  bool ok_a, ok_b;
+  if (d.a_kcontig) {
     ok_a = make_tensor_map_f64(&L.ma, d.A, d.M, d.K, BK, plan.bm, lda);
   } else if (lda % 16 == 0 && make_tensor_map_f64_grouped(&L.ma, d.A, d.K, lda, BK, plan.bm / 16)) {
+    ok_a = true;
     L.grouped_ab |= 1;
   } else {
     ok_a = make_tensor_map_f64(&L.ma, d.A, d.K, d.M, 16, BK, lda);
@@ -134,7 +142,6 @@ int run_gemm_ext(const GemmExt &e) {
     ok_b = make_tensor_map_f64(&L.mb, d.B, d.K, d.N, 16, BK, ldb);
   }
   if (!ok_a || !ok_b) return fail(MG_ERR_CUDA, "gemm: cuTensorMapEncodeTiled failed");
-  if (q8) L.ma = L.mb;
   L.mmask = L.mb;
 
   GemmEpilogue ep{};
@@ -163,13 +170,19 @@ int run_gemm_ext(const GemmExt &e) {
   L.M = M; L.N = N; L.K = K;
   L.tiles_m = tiles_m; L.tiles_n = tiles_n;
   L.table = table ? table->dev_items : nullptr;
-  L.tickets = table && table->slots > 0 ? table->dev_tickets : nullptr;
+  const bool split = table && table->slots > 0, fold_here = split && plan.spans >= kFoldBySegments * tiles_m * tiles_n;
+  L.tickets = split && !fold_here ? table->dev_tickets : nullptr;
   L.items = table ? table->items : tiles_m * tiles_n;
   L.min_nkt = table ? table->min_nkt : KT;
-  if (q8) return launch_q8(plan.tile, L);
-  if (d.a_kcontig && !d.b_kcontig) return launch_layout_ext<true, false>(plan.tile, L);
-  if (d.a_kcontig) return launch_layout_ext<true, true>(plan.tile, L);
-  return launch_layout_ext<false, false>(plan.tile, L);
+  int rc;
+  if (d.a_kcontig && !d.b_kcontig) rc = launch_layout_ext<true, false>(plan.tile, L);
+  else if (d.a_kcontig) rc = launch_layout_ext<true, true>(plan.tile, L);
+  else rc = launch_layout_ext<false, false>(plan.tile, L);
+  if (rc != MG_OK || !fold_here) return rc;
+  fold_tiles_kernel<<<dim3((unsigned)((plan.bm * plan.bn + 255) / 256), (unsigned)(tiles_m * tiles_n)), 256, 0,
+                      c.stream>>>(ep, table->dev_tiles, tiles_n, plan.bm, plan.bn, M, N);
+  MG_LAUNCH_CHECK("gemm fold");
+  return MG_OK;
 }
 
 }  // namespace mg

@@ -1,6 +1,6 @@
 // The FP64 tensor-core GEMM kernel, its tile configurations and its launch.  gemm.cu
 // describes the design and instantiates it for the dense products; gemm_ext.cu does so
-// for few rows, row pitches, odd row lengths and 8-bit operands.
+// for few rows, row pitches, odd row lengths and 8-bit masks.
 #pragma once
 
 #include "common.cuh"
@@ -15,8 +15,6 @@ constexpr int kProducerWarps = 4;  // one warp group; only its first lane issues
 constexpr int kGemmThreads = (kConsumerWarps + kProducerWarps) * 32;  // 384
 // Register split between the warp groups (setmaxnreg): 8*32*232 + 4*32*40 <= 64 K.
 constexpr int kConsumerRegs = 232, kProducerRegs = 40;
-// With a producer group that converts 8-bit codes: 8*32*224 + 4*32*56, the same sum.
-constexpr int kConsumerRegsQ8 = 224, kProducerRegsQ8 = 56;
 
 // CTA tile = (8 / WARPS_N) x WARPS_N consumer warps, each owning MT x NT
 // sub-tiles of 16 x 8 outputs.
@@ -82,31 +80,6 @@ struct GemmEpilogue {
   size_t ld_mask8;
   int pairs;                 // D's rows all start on 16-byte boundaries
 };
-
-// Scales of a stage of 8-bit codes: its 16 rows, for each of the tile's two blocks.
-constexpr int kQ8StageScales = 2 * BK;
-
-// The A operand of a transposed-A product in 8 bits (Q8A instantiations): codes
-// [K][ldc] (base and pitch multiples of 16 bytes) and one scale per 64 columns of a row,
-// [K][blocks].
-struct Q8Operand {
-  const signed char *codes;
-  const double *scales;
-  size_t ldc, blocks;
-  int cols;  // columns of the codes, = M of the product
-};
-
-// Byte e of a word of codes, each with its top bit flipped (0 .. 255 for -128 .. 127), as
-// the high word of the double it stands for (the low word is 0).  The fp64 units are
-// left to the tensor instructions, behind which every fp64 instruction would queue: the
-// byte becomes the low end of the float 2^23 + byte, 2^23 + 128 is taken from that in
-// fp32 (exact), and the float's sign, exponent and fraction move to their places in a
-// double.
-__device__ __forceinline__ int widen_code(unsigned flipped, int e) {
-  const float f = __uint_as_float(__byte_perm(flipped, 0x4b000000u, 0x7540 + e)) - 8388736.0f;
-  const unsigned bits = __float_as_uint(f), wide = ((bits >> 3) & 0x0fffffffu) + 0x38000000u;
-  return (int)(f == 0.0f ? 0u : (wide | (bits & 0x80000000u)));
-}
 
 // Fragment pair (k = 2c, 2c+1) of the A operand for the MT row sub-tiles of a
 // warp: lo = rows g, hi = rows g + 8 of each 16-row sub-tile.
@@ -205,41 +178,15 @@ __device__ __forceinline__ void compute_stage(double (&acc)[MT][NT][4], const ui
   }
 }
 
-// The same with A = codes (transposed-A layout): the scale of a contraction row goes to
-// the B fragments instead, a multiplication for every 8 MT MMA rows.  The MT row
-// sub-tiles of a warp lie in one 64-column block of the codes; sc = its 16 scales.
-template <int MT, int NT>
-__device__ __forceinline__ void compute_stage_q8(double (&acc)[MT][NT][4], const uint8_t *As, const uint8_t *Bs,
-                                                 const double *sc, int c0, int g, int wm, int wn) {
-#pragma unroll
-  for (int slab = 0; slab < 2; slab++) {
-    double2 lo[MT], hi[MT], b[NT];
-    const double2 s = *reinterpret_cast<const double2 *>(sc + 2 * (c0 ^ slab));
-    load_a_frags<false, MT>(As, c0 ^ slab, g, wm, lo, hi);
-    load_b_frags<false, NT>(Bs, c0 ^ slab, g, wn, b);
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-      b[nt].x *= s.x;
-      b[nt].y *= s.y;
-    }
-#pragma unroll
-    for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-      for (int nt = 0; nt < NT; nt++)
-        dmma_m16n8k8(acc[mt][nt], lo[mt].x, hi[mt].x, lo[mt].y, hi[mt].y, b[nt].x, b[nt].y);
-  }
-}
-
 // Consumer side of the stage ring: wait for a stage, run its MMAs, hand the
 // stage back.  `active` is false for a warp whose whole sub-block lies outside
 // the matrix (ragged border tiles): it skips the arithmetic but keeps the
 // barrier protocol.  Returns false if a bounded wait gave up.
-template <bool A_KCONTIG, bool B_KCONTIG, int SHAPE, class Cfg, bool Q8A = false>
+template <bool A_KCONTIG, bool B_KCONTIG, int SHAPE, class Cfg>
 __device__ __forceinline__ bool consumer_loop(double (&acc)[Cfg::MT][Cfg::NT][4], const uint8_t *smem,
                                               uint64_t *full_bar, uint64_t *empty_bar, int nkt,
                                               unsigned &ring, volatile int *abort_flag, int c0, int g,
-                                              int wm, int wn, int lane, bool active,
-                                              const double *scales = nullptr) {
+                                              int wm, int wn, int lane, bool active) {
   // `ring` counts stages consumed by this CTA since it started; it runs on across
   // the tiles a persistent CTA processes, so stage index and barrier phase follow.
   for (int it = 0; it < nkt; ++it, ++ring) {
@@ -247,10 +194,7 @@ __device__ __forceinline__ bool consumer_loop(double (&acc)[Cfg::MT][Cfg::NT][4]
     if (!mbar_wait_bounded(smem_u32(full_bar + s), (ring / Cfg::STAGES) & 1, abort_flag)) return false;
     const uint8_t *As = smem + s * Cfg::STAGE_BYTES;
     const uint8_t *Bs = As + Cfg::A_BYTES;
-    if (Q8A) {
-      if (active)
-        compute_stage_q8<Cfg::MT, Cfg::NT>(acc, As, Bs, scales + s * kQ8StageScales + (wm >> 6) * BK, c0, g, wm, wn);
-    } else if (active)
+    if (active)
       compute_stage<A_KCONTIG, B_KCONTIG, SHAPE, Cfg::MT, Cfg::NT>(acc, As, Bs, c0, g, wm, wn);
     __syncwarp();
     if (lane == 0) mbar_arrive(smem_u32(empty_bar + s));
@@ -324,18 +268,14 @@ __device__ __forceinline__ WorkItem decode_work(int id, int tiles_n, int KT,
 // final epilogue itself, so no second kernel is needed and the fold of one tile
 // overlaps the other CTAs' MMAs.
 // ANYD: the output has a row pitch, rows of odd length or a ReLU mask in 8 bits.
-// Q8A: the A operand (of a transposed-A product) comes in 8 bits; the producer group's
-// 128 threads read the codes some k-tiles ahead, widen them to whole doubles and store
-// them where TMA would have put the fp64 tile, and hand the rows' scales to the
-// consumers, which multiply the other operand by them.
 template <bool A_KCONTIG, bool B_KCONTIG, int SHAPE, bool EDGE, class Cfg, bool PERSISTENT, bool MASKED,
-          bool FOLD, bool ANYD = false, bool Q8A = false>
+          bool FOLD, bool ANYD = false>
 __global__ void __launch_bounds__(kGemmThreads, 1)
 dmma_gemm_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB,
                  const __grid_constant__ CUtensorMap mapMask, GemmEpilogue ep, int M, int N, int K,
                  int tiles_n, const SegItem *__restrict__ table, int grouped_ab, int total_items,
-                 unsigned int *tile_tickets, int *status, Q8Operand qa) {
-  static_assert(!(MASKED && (ANYD || Q8A)) && !(Q8A && (A_KCONTIG || Cfg::BM != 128)), "no such variant");
+                 unsigned int *tile_tickets, int *status) {
+  static_assert(!(MASKED && ANYD), "no such variant");
   constexpr int BM = Cfg::BM, BN = Cfg::BN, MT = Cfg::MT, NT = Cfg::NT;
   constexpr int kStages = Cfg::STAGES, kStageBytes = Cfg::STAGE_BYTES, kTileBytes = Cfg::A_BYTES;
   extern __shared__ uint8_t smem_raw[];
@@ -349,7 +289,6 @@ dmma_gemm_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant
   uint64_t *empty_bar = full_bar + kStages;
   uint64_t *fold_bar = full_bar + 2 * kStages;  // consumer warps meet here around the tile ticket
   static_assert(2 * kStages + 1 == Cfg::kBarriers, "barrier area and its users out of step");
-  double *q8_scales = Q8A ? reinterpret_cast<double *>(full_bar + (Cfg::kBarriers + 1) / 2 * 2) : nullptr;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int KT = (K + BK - 1) / BK;
@@ -357,7 +296,7 @@ dmma_gemm_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant
   if (threadIdx.x == 0) {
     abort_flag_s = 0;
     for (int s = 0; s < kStages; s++) {
-      mbar_init(smem_u32(full_bar + s), Q8A ? 1 + kProducerWarps : 1);
+      mbar_init(smem_u32(full_bar + s), 1);
       mbar_init(smem_u32(empty_bar + s), kConsumerWarps);
     }
     mbar_init(smem_u32(fold_bar), kConsumerWarps);
@@ -367,81 +306,6 @@ dmma_gemm_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant
 
   if (warp >= kConsumerWarps) {
     // ---------------- producer warp group: one lane drives the TMA ring ----------------
-    if constexpr (Q8A) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegsQ8));
-      const int pt = threadIdx.x - kConsumerWarps * 32;
-      // A thread widens 16 codes of one row.  Eight rows to a warp: the rows differ in
-      // the swizzle, so a warp's 16-byte stores spread over all banks.
-      const int r = (pt & 7) | ((pt >> 6) << 3), j = (pt >> 3) & 7;
-      if (pt == 0) prefetch_tensormap(&mapB);
-      constexpr int kAhead = 4;
-      unsigned ring = 0;
-      bool alive = true;
-      int id = blockIdx.x;
-      do {
-        const WorkItem w = decode_work<Cfg>(id, tiles_n, KT, table);
-        const int col = w.m0 + 16 * j;
-        // Loads are never conditional (a value merged with a default is waited for at the
-        // merge): outside the operand they read its last row or column group, and the
-        // value is dropped when it is widened.
-        int4 code[kAhead];
-        double scale[kAhead];
-        const int col_in = min(col, qa.cols - 1) & ~15;
-        const signed char *codes = qa.codes + col_in;
-        const double *scales = qa.scales + (col_in >> 6);
-        auto read = [&](int it, int4 &c, double &s) {
-          const int row = min((w.kt_begin + it) * BK + r, K - 1);
-          s = __ldg(scales + (size_t)row * qa.blocks);
-          c = __ldg(reinterpret_cast<const int4 *>(codes + (size_t)row * qa.ldc));
-        };
-#pragma unroll
-        for (int u = 0; u < kAhead; u++) read(u, code[u], scale[u]);
-        for (int it0 = 0; it0 < w.nkt && alive; it0 += kAhead) {
-#pragma unroll
-          for (int u = 0; u < kAhead; u++) {
-            const int it = it0 + u;
-            if (it < w.nkt && alive) {
-              const unsigned s = ring % kStages;
-              if (ring >= (unsigned)kStages)
-                alive = mbar_wait_bounded(smem_u32(empty_bar + s), ((ring / kStages) - 1) & 1, abort_flag);
-              if (alive) {
-                const uint32_t bar = smem_u32(full_bar + s);
-                uint8_t *stage = smem + s * kStageBytes;
-                if (pt == 0) {
-                  mbar_arrive_expect_tx(bar, Cfg::B_BYTES);
-                  const uint32_t b_dst = smem_u32(stage) + kTileBytes;
-                  const int k0 = (w.kt_begin + it) * BK;
-                  if (grouped_ab & 2) {
-                    tma_load_3d(b_dst, &mapB, 0, k0, w.n0 >> 4, bar);
-                  } else {
-                    for (int b = 0; b < BN / 16; b++)
-                      tma_load_2d(b_dst + b * 2048, &mapB, w.n0 + 16 * b, k0, bar);
-                  }
-                }
-                uint8_t *dst = stage + j * 2048 + r * 128;
-                const bool in = (w.kt_begin + it) * BK + r < K && col < qa.cols;
-                // (the threads of a block's first 16 columns pass its scale on)
-                if ((j & 3) == 0) q8_scales[s * kQ8StageScales + (j >> 2) * BK + r] = in ? scale[u] : 0.0;
-                const unsigned none = 0x80808080u;
-                const unsigned word[4] = {in ? (unsigned)code[u].x ^ none : none, in ? (unsigned)code[u].y ^ none : none,
-                                          in ? (unsigned)code[u].z ^ none : none, in ? (unsigned)code[u].w ^ none : none};
-#pragma unroll
-                for (int c = 0; c < 8; c++)
-                  *reinterpret_cast<int4 *>(dst + ((c ^ (r & 7)) << 4)) =
-                      make_int4(0, widen_code(word[c >> 1], 2 * (c & 1)), 0,
-                                widen_code(word[c >> 1], 2 * (c & 1) + 1));
-                __syncwarp();
-                if ((pt & 31) == 0) mbar_arrive(bar);
-                ring++;
-                read(it + kAhead, code[u], scale[u]);
-              }
-            }
-          }
-        }
-        if (!PERSISTENT) break;
-        id += gridDim.x;
-      } while (alive && id < total_items);
-    } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
     if (warp == kConsumerWarps && lane == 0) {
       prefetch_tensormap(&mapA);
@@ -506,10 +370,9 @@ dmma_gemm_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant
         id += gridDim.x;
       } while (alive && id < total_items);
     }
-    }  // !Q8A
   } else {
     // ---------------- consumer warp groups ----------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Q8A ? kConsumerRegsQ8 : kConsumerRegs));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kConsumerRegs));
     const int g = lane >> 2, t = lane & 3;
     const int wm = (warp / Cfg::WARPS_N) * (MT * 16), wn = (warp % Cfg::WARPS_N) * (NT * 8);
     // 16-byte chunk owned by this thread in the first half-slab; the second
@@ -537,8 +400,8 @@ dmma_gemm_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant
       // instruction stream.)  Out-of-range rows and columns of a live warp read
       // zeros from the TMA fill and are dropped in the epilogue.
       const bool active = !EDGE || (M > m0 + wm && N > n0 + wn);
-      const bool ok = consumer_loop<A_KCONTIG, B_KCONTIG, SHAPE, Cfg, Q8A>(
-          acc, smem, full_bar, empty_bar, w.nkt, ring, abort_flag, c0, g, wm, wn, lane, active, q8_scales);
+      const bool ok = consumer_loop<A_KCONTIG, B_KCONTIG, SHAPE, Cfg>(
+          acc, smem, full_bar, empty_bar, w.nkt, ring, abort_flag, c0, g, wm, wn, lane, active);
       if (!ok) break;
       // Mask source staged by the producer: wait for all of its stages (every warp,
       // also an inactive one, keeps the ring's barrier protocol).
@@ -824,18 +687,16 @@ struct DmmaLaunch {
   int items;             // CTAs' worth of work: segments, or tiles
   int min_nkt;           // shortest item, in k-tiles
   int grouped_ab;  // bit 0 / bit 1: operand A / B uses the grouped 3-D tensor map
-  Q8Operand qa;    // Q8A instantiations: operand A
 };
 
 template <bool AK, bool BK_, int SHAPE, bool EDGE, class Cfg, bool PERSISTENT, bool MASKED, bool FOLD,
-          bool ANYD = false, bool Q8A = false>
+          bool ANYD = false>
 static int launch_dmma_masked(const DmmaLaunch &L) {
   static bool configured = false;
-  constexpr int kSmem = Cfg::SMEM_BYTES + (Q8A ? 16 + Cfg::STAGES * kQ8StageScales * 8 : 0);
-  static_assert(kSmem <= 227 * 1024, "more shared memory than a CTA can have");
-  auto kernel = dmma_gemm_kernel<AK, BK_, SHAPE, EDGE, Cfg, PERSISTENT, MASKED, FOLD, ANYD, Q8A>;
+  auto kernel = dmma_gemm_kernel<AK, BK_, SHAPE, EDGE, Cfg, PERSISTENT, MASKED, FOLD, ANYD>;
   if (!configured) {
-    MG_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    MG_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     Cfg::SMEM_BYTES));
     configured = true;
   }
   Context &c = ctx();
@@ -844,9 +705,9 @@ static int launch_dmma_masked(const DmmaLaunch &L) {
   // run as a persistent grid, where the cross-item prefetch hides the pipeline
   // fill that would otherwise dominate them.
   dim3 grid((unsigned)((PERSISTENT && L.items > c.sm_count) ? c.sm_count : L.items), 1, 1);
-  kernel<<<grid, kGemmThreads, kSmem, c.stream>>>(L.ma, L.mb, L.mmask, L.ep, L.M, L.N, L.K,
+  kernel<<<grid, kGemmThreads, Cfg::SMEM_BYTES, c.stream>>>(L.ma, L.mb, L.mmask, L.ep, L.M, L.N, L.K,
                                                              L.tiles_n, L.table, L.grouped_ab,
-                                                             L.items, L.tickets, c.kernel_status, L.qa);
+                                                             L.items, L.tickets, c.kernel_status);
   MG_LAUNCH_CHECK("dmma_gemm");
   return MG_OK;
 }
@@ -869,6 +730,7 @@ struct SegTable {
   int items, slots, min_nkt;
   SegItem *dev_items;  // [items], longest first
   unsigned int *dev_tickets;  // [tiles]: arrival counters of the in-kernel fold, zero between launches
+  int2 *dev_tiles;            // [tiles]: first slot and segment count of a split tile, (0, 0) of a whole one
 };
 
 int choose_spans(int tiles, int KT, int sms);

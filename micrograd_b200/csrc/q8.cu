@@ -130,14 +130,14 @@ q8_pack_kernel(const double *__restrict__ x, signed char *__restrict__ codes, do
 template <int VEC, int UN, bool FLAT>
 __global__ void __launch_bounds__(kQ8Threads)
 q8_unpack_kernel(const signed char *__restrict__ codes, const double *__restrict__ scales,
-                 double *__restrict__ x, size_t blocks, size_t N, unsigned nb) {
+                 double *__restrict__ x, size_t pitch, size_t blocks, size_t N, unsigned nb) {
   constexpr int LANES = VEC == 4 ? 16 : 32, PER = 64 / LANES;
   const int lane = threadIdx.x % LANES;
   const size_t teams = (size_t)gridDim.x * (kQ8Threads / LANES);
   for (size_t b0 = ((size_t)blockIdx.x * kQ8Threads + threadIdx.x) / LANES; b0 < blocks; b0 += teams * UN) {
     unsigned word[UN];
     double scale[UN];
-    size_t at[UN];
+    size_t at[UN], to[UN];
     int cols[UN];
 #pragma unroll
     for (int u = 0; u < UN; u++) {
@@ -146,12 +146,13 @@ q8_unpack_kernel(const signed char *__restrict__ codes, const double *__restrict
       word[u] = 0;
       if (b < blocks) {
         if (FLAT) {
-          at[u] = b * 64 + lane * PER;
+          at[u] = to[u] = b * 64 + lane * PER;
           cols[u] = PER;
         } else {
           const size_t row = blocks >> 32 ? b / nb : (size_t)((unsigned)b / nb);
           const size_t c = (b - row * nb) * 64 + lane * PER;
           at[u] = row * N + c;
+          to[u] = row * pitch + c;
           cols[u] = c < N ? (N - c < PER ? (int)(N - c) : PER) : 0;
         }
       }
@@ -174,17 +175,19 @@ q8_unpack_kernel(const signed char *__restrict__ codes, const double *__restrict
 #pragma unroll
       for (int k = 0; k < PER; k++) v[k] = (double)(signed char)(word[u] >> (8 * k)) * scale[u];
       if constexpr (VEC == PER && PER == 4) {
-        st_stream_v4(reinterpret_cast<double4v *>(x + at[u]), double4v{v[0], v[1], v[2], v[3]});
+        st_stream_v4(reinterpret_cast<double4v *>(x + to[u]), double4v{v[0], v[1], v[2], v[3]});
       } else if constexpr (VEC == PER) {
-        __stcs(reinterpret_cast<double2 *>(x + at[u]), make_double2(v[0], v[1]));
+        __stcs(reinterpret_cast<double2 *>(x + to[u]), make_double2(v[0], v[1]));
       } else {
 #pragma unroll
         for (int k = 0; k < PER; k++)
-          if (k < cols[u]) x[at[u] + k] = v[k];
+          if (k < cols[u]) x[to[u] + k] = v[k];
       }
     }
   }
 }
+
+static size_t q8_blocks(size_t N) { return (N + kQ8Block - 1) / kQ8Block; }
 
 // gx (+)= g where the code is positive: the gradient of a ReLU whose input or output
 // is kept in 8 bits.
@@ -206,99 +209,143 @@ static int q8_vec(const double *x, const signed char *codes, size_t N) {
   return 1;
 }
 
-static size_t q8_blocks(size_t N) { return (N + kQ8Block - 1) / kQ8Block; }
 
-// dst[rows][pitch] = src[rows][cols], zeros behind them (pitch a multiple of 16).
-__global__ void __launch_bounds__(256)
-q8_copy_rows_kernel(const signed char *__restrict__ src, size_t rows, size_t cols, signed char *__restrict__ dst,
-                    size_t pitch) {
-  const size_t words = pitch / 4, all = rows * words;
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (size_t)gridDim.x * 256) {
-    const size_t r = all >> 32 ? i / words : (size_t)((unsigned)i / (unsigned)words), c = (i - r * words) * 4;
-    const signed char *p = src + r * cols + c;
-    unsigned w = 0;
-#pragma unroll
-    for (int k = 0; k < 4; k++)
-      if (c + k < cols) w |= (unsigned)(unsigned char)p[k] << (8 * k);
-    reinterpret_cast<unsigned *>(dst)[i] = w;
+// ---------------------------------------------------------------------------
+// Products with few columns (N <= 32): streams of one byte per element for 2 N flop.
+// The tensor kernel would need the fp64 form of the codes, 8 bytes each, written and
+// read, or spend its tiles on padding.  These keep the narrow operand's values (or the
+// sums) of two columns per lane in registers; tiles of codes and the rows of G that go
+// with them come through a ring of kRing stages in shared memory by asynchronous copies.
+// ---------------------------------------------------------------------------
+constexpr int kRing = 3;
+
+__device__ __forceinline__ uint32_t shared_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// 8 bytes, or zeros.
+__device__ __forceinline__ void copy8(void *dst, const void *src, bool in) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(shared_address(dst)), "l"(src), "r"(in ? 8 : 0)
+               : "memory");
+}
+
+// Rows m0 .. m0 + rows - 1 of G[M][N] into dst[rows][NN] (its last column is left alone
+// where N is odd, rows from M on become zeros), by the CTA's `threads` threads.  Even N
+// from a 16-byte boundary: the rows are one run of memory on both sides.
+template <int NN>
+__device__ __forceinline__ void copy_g(double *dst, const double *__restrict__ G, size_t m0, size_t M, int rows, int N,
+                                       int tid, int threads, bool run) {
+  const double *src = G + m0 * N;
+  if (run) {
+    const int in = M > m0 ? (M - m0 < (size_t)rows ? (int)(M - m0) : rows) * N : 0;  // values that exist
+    for (int i = 2 * tid; i < rows * NN; i += 2 * threads)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(shared_address(dst + i)),
+                   "l"(i < in ? src + i : G), "r"(i < in ? 16 : 0)
+                   : "memory");
+  } else {
+    for (int i = tid; i < rows * N; i += threads) {
+      const int r = i / N;
+      const bool in = m0 + r < M;
+      copy8(dst + r * NN + (i - r * N), in ? src + i : G, in);
+    }
   }
 }
 
-static int copy_codes_rows(const signed char *src, size_t rows, size_t cols, signed char *dst, size_t pitch) {
-  q8_copy_rows_kernel<<<grid_for(rows * pitch / 4, 256, 32), 256, 0, ctx().stream>>>(src, rows, cols, dst, pitch);
-  MG_LAUNCH_CHECK("copy of codes");
-  return MG_OK;
+// How the rows of a matrix of codes can be read: 16 or 4 bytes at a time, or single ones.
+enum { kCodes16, kCodes4, kCodes1 };
+static int code_access(const signed char *codes, size_t K) {
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(codes) | K;
+  return bits % 16 == 0 ? kCodes16 : (bits % 4 == 0 ? kCodes4 : kCodes1);
 }
 
-// dA[M][K] (+)= (G[M][N] . B[K][N]^T) * (mask > 0) for N <= 16: nothing but streaming
-// the output, 9 bytes per element (17 when accumulating) against 2 N flop.  A thread
-// keeps two columns' rows of B in registers and walks down the rows; the rows of G pass
-// through shared memory, where a warp reads each value once for its 64 outputs.
-// PAIR: the two columns are neighbours (K even, aligned), else TX apart.  The next
-// rows of G and of the mask are on their way while a block of rows is computed.
-constexpr int kOuterRows = 8;  // rows per thread and block
+// The 16 codes from column `col` of row m on into dst (16-byte aligned), zeros outside.
+template <int ACCESS>
+__device__ __forceinline__ void copy_codes(uint8_t *dst, const signed char *__restrict__ codes, size_t m, size_t M,
+                                           size_t col, size_t K) {
+  const bool row = m < M;
+  const signed char *src = codes + (row ? m * K : 0);
+  if (ACCESS == kCodes16) {
+    const bool in = row && col < K;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(shared_address(dst)), "l"(in ? src + col : src),
+                 "r"(in ? 16 : 0)
+                 : "memory");
+  } else if (ACCESS == kCodes4) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const bool in = row && col + 4 * k < K;
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(shared_address(dst + 4 * k)),
+                   "l"(in ? src + col + 4 * k : src), "r"(in ? 4 : 0)
+                   : "memory");
+    }
+  } else {
+    unsigned word[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int k = 0; k < 16; k++)
+      if (row && col + k < K) word[k >> 2] |= (unsigned)(unsigned char)src[col + k] << (8 * (k & 3));
+    *reinterpret_cast<uint4 *>(dst) = make_uint4(word[0], word[1], word[2], word[3]);
+  }
+}
 
-template <int NN, bool PAIR>
-__global__ void __launch_bounds__(256, 2)
+// dA[M][K] (+)= (G[M][N] . B[K][N]^T) * (mask > 0), N <= 16: nothing but streaming the
+// output, 9 bytes per element (17 when accumulating).  TX x TY threads take 2 TX columns
+// of 8 TY rows at a time.  PAIR: the two columns of a thread are neighbours (K even,
+// dA aligned), else TX apart.
+constexpr int kOuterRows = 8;  // rows per thread and tile
+constexpr int kOuterCodes = 256 * 2 * kOuterRows;  // codes of a tile
+
+template <int NN, bool PAIR, int ACCESS>
+__global__ void __launch_bounds__(256, NN <= 8 ? 4 : 3)
 q8_outer_kernel(const double *__restrict__ G, const double *__restrict__ B, double *dA,
                 const signed char *__restrict__ mask, size_t M, int N, size_t K, bool accumulate) {
-  constexpr int kMostTY = 8, kPer = (kOuterRows * kMostTY * NN + 255) / 256;
-  __shared__ __align__(16) double gs[2][kOuterRows * kMostTY * NN];
+  constexpr int kMostRows = kOuterRows * 8;
+  __shared__ __align__(16) double gs[kRing][kMostRows * NN];
+  __shared__ __align__(16) uint8_t cs[kRing][kOuterCodes];
   const int TX = blockDim.x, TY = blockDim.y, tid = threadIdx.y * TX + threadIdx.x;
-  const size_t c0 = (size_t)blockIdx.x * 2 * TX + (PAIR ? 2 * threadIdx.x : threadIdx.x), c1 = PAIR ? c0 + 1 : c0 + TX;
-  const bool in0 = c0 < K, in1 = c1 < K;
+  const int width = 2 * TX, rows = kOuterRows * TY, mine = PAIR ? 2 * threadIdx.x : threadIdx.x, apart = PAIR ? 1 : TX;
+  const size_t col0 = (size_t)blockIdx.x * width, c0 = col0 + mine;
+  const bool in0 = c0 < K, in1 = c0 + apart < K;
+  const size_t tiles = (M + rows - 1) / rows;
+  const int chunks = width / 16, my_row = tid / chunks, my_col = (tid - my_row * chunks) * 16;
+  if (N < NN)  // (an odd N: the last value of a staged row stays 0)
+    for (int i = tid; i < kRing * rows; i += 256) gs[i / rows][(i % rows) * NN + N] = 0.0;
+  const bool run = N == NN && (reinterpret_cast<uintptr_t>(G) & 15) == 0;
+  auto fetch = [&](size_t tile, int stage) {
+    if (tile < tiles) {
+      const size_t m0 = tile * rows;
+      copy_codes<ACCESS>(&cs[stage][my_row * width + my_col], mask, m0 + my_row, M, col0 + my_col, K);
+      copy_g<NN>(gs[stage], G, m0, M, rows, N, tid, 256, run);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
   double b0[NN], b1[NN];
 #pragma unroll
   for (int n = 0; n < NN; n++) {
     b0[n] = in0 && n < N ? B[c0 * N + n] : 0.0;
-    b1[n] = in1 && n < N ? B[c1 * N + n] : 0.0;
+    b1[n] = in1 && n < N ? B[(c0 + apart) * N + n] : 0.0;
   }
-  const int rows = kOuterRows * TY, values = rows * NN;
-  const size_t blocks = (M + rows - 1) / rows;
-  unsigned short next[kOuterRows];  // a row's two codes
-  double g_next[kPer];
-  auto read = [&](size_t blk) {
-    const size_t m0 = blk * rows;
+  size_t tile = blockIdx.y;
 #pragma unroll
-    for (int u = 0; u < kOuterRows; u++) {
-      const size_t m = m0 + u * TY + threadIdx.y, at = m * K;
-      next[u] = 0;
-      if (m < M) {
-        if (PAIR) {
-          if (in0) next[u] = __ldcs(reinterpret_cast<const unsigned short *>(mask + at + c0));
-        } else {
-          if (in0) next[u] = (unsigned char)mask[at + c0];
-          if (in1) next[u] |= (unsigned short)((unsigned char)mask[at + c1] << 8);
-        }
+  for (int s = 0; s < kRing - 1; s++) fetch(tile + s * (size_t)gridDim.y, s);
+  const size_t step = (size_t)TY * K;
+  int stage = 0;
+  for (; tile < tiles; tile += gridDim.y) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
+    __syncthreads();  // the stage is complete, and the one before it is read no more
+    fetch(tile + (kRing - 1) * (size_t)gridDim.y, stage == 0 ? kRing - 1 : stage - 1);
+    const size_t m0 = tile * rows;
+    const int left = (int)(M - m0 < (size_t)rows ? M - m0 : rows);
+    double *dst = dA + (m0 + threadIdx.y) * K + c0;
+    const double *g = &gs[stage][threadIdx.y * NN];
+    const uint8_t *code = &cs[stage][threadIdx.y * width + mine];
+#pragma unroll 2
+    for (int r = threadIdx.y; r < left; r += TY, dst += step, g += TY * NN, code += TY * width) {
+      int k0, k1;
+      if (PAIR) {
+        const short two = *reinterpret_cast<const short *>(code);
+        k0 = (signed char)two;
+        k1 = two >> 8;
+      } else {
+        k0 = (signed char)code[0];
+        k1 = (signed char)code[apart];
       }
-    }
-#pragma unroll
-    for (int k = 0; k < kPer; k++) {
-      const int i = tid + 256 * k, r = i / NN, n = i % NN;
-      g_next[k] = i < values && m0 + r < M && n < N ? __ldg(G + (m0 + r) * N + n) : 0.0;
-    }
-  };
-  auto hand_over = [&](int buf) {
-#pragma unroll
-    for (int k = 0; k < kPer; k++)
-      if (tid + 256 * k < values) gs[buf][tid + 256 * k] = g_next[k];
-  };
-  size_t blk = blockIdx.y;
-  if (blk < blocks) read(blk);
-  hand_over(0);
-  int buf = 0;
-  for (; blk < blocks; blk += gridDim.y, buf ^= 1) {
-    __syncthreads();  // gs[buf] is complete, and nobody reads the other one any more
-    unsigned short codes[kOuterRows];
-#pragma unroll
-    for (int u = 0; u < kOuterRows; u++) codes[u] = next[u];
-    if (blk + gridDim.y < blocks) read(blk + gridDim.y);
-#pragma unroll
-    for (int u = 0; u < kOuterRows; u++) {
-      const int r = u * TY + threadIdx.y;
-      const size_t m = blk * rows + r;
-      if (m >= M) continue;
-      const double *g = &gs[buf][r * NN];
       double s0 = 0.0, s1 = 0.0;
 #pragma unroll
       for (int n = 0; n < NN; n += 2) {
@@ -308,48 +355,223 @@ q8_outer_kernel(const double *__restrict__ G, const double *__restrict__ B, doub
         s0 = fma(v.y, b0[n + 1], s0);
         s1 = fma(v.y, b1[n + 1], s1);
       }
-      s0 = s0 * ((signed char)codes[u] > 0 ? 1.0 : 0.0);
-      s1 = s1 * ((short)codes[u] >= 256 ? 1.0 : 0.0);  // (its high byte > 0)
-      double *dst = dA + m * K;
+      s0 = s0 * (k0 > 0 ? 1.0 : 0.0);
+      s1 = s1 * (k1 > 0 ? 1.0 : 0.0);
       if (PAIR) {
         if (!in0) continue;
         if (accumulate) {
-          const double2 o = *reinterpret_cast<const double2 *>(dst + c0);
+          const double2 o = *reinterpret_cast<const double2 *>(dst);
           s0 = o.x + s0;
           s1 = o.y + s1;
         }
-        __stcs(reinterpret_cast<double2 *>(dst + c0), make_double2(s0, s1));
+        __stcs(reinterpret_cast<double2 *>(dst), make_double2(s0, s1));
       } else {
-        if (in0) dst[c0] = accumulate ? dst[c0] + s0 : s0;
-        if (in1) dst[c1] = accumulate ? dst[c1] + s1 : s1;
+        if (in0) dst[0] = accumulate ? dst[0] + s0 : s0;
+        if (in1) dst[apart] = accumulate ? dst[apart] + s1 : s1;
       }
     }
-    hand_over(buf ^ 1);
+    stage = stage + 1 == kRing ? 0 : stage + 1;
   }
+}
+
+template <int NN>
+static void launch_outer(dim3 grid, dim3 block, bool pair, int access, const double *G, const double *B, double *dA,
+                         const signed char *mask, size_t M, int N, size_t K, bool acc) {
+  cudaStream_t s = ctx().stream;
+  if (pair && access == kCodes16) q8_outer_kernel<NN, true, kCodes16><<<grid, block, 0, s>>>(G, B, dA, mask, M, N, K, acc);
+  else if (pair && access == kCodes4) q8_outer_kernel<NN, true, kCodes4><<<grid, block, 0, s>>>(G, B, dA, mask, M, N, K, acc);
+  else if (pair) q8_outer_kernel<NN, true, kCodes1><<<grid, block, 0, s>>>(G, B, dA, mask, M, N, K, acc);
+  else q8_outer_kernel<NN, false, kCodes1><<<grid, block, 0, s>>>(G, B, dA, mask, M, N, K, acc);
 }
 
 static int outer_q8(const double *G, const double *B, double *dA, size_t M, size_t N, size_t K, int accumulate,
                     const signed char *mask) {
   unsigned tx = 32;
   while (tx < 256 && 2 * (size_t)tx < K) tx *= 2;
-  const bool pair = K % 2 == 0 && !off_16_bytes(dA) && !(reinterpret_cast<uintptr_t>(mask) & 1);
-  const size_t rows = (size_t)kOuterRows * (256 / tx), gx = (K + 2 * tx - 1) / (2 * tx), blocks = (M + rows - 1) / rows;
-  size_t gy = (size_t)ctx().sm_count * 16 / gx + 1;
-  if (gy > blocks) gy = blocks;
-  if (gy > 65535) gy = 65535;
+  const bool pair = K % 2 == 0 && !off_16_bytes(dA);
+  const int access = code_access(mask, K);
+  const size_t rows = (size_t)kOuterRows * (256 / tx), gx = (K + 2 * tx - 1) / (2 * tx), tiles = (M + rows - 1) / rows;
+  // (one wave: a CTA's start, its rows of B, costs as much as several tiles)
+  size_t gy = (size_t)ctx().sm_count * (N <= 8 ? 4 : 3) / gx;
+  if (gy < 1) gy = 1;
+  if (gy > tiles) gy = tiles;
   const dim3 grid((unsigned)gx, (unsigned)gy), block(tx, 256 / tx);
-  cudaStream_t stream = ctx().stream;
-#define MG_OUTER(NN)                                                                                        \
-  (pair ? q8_outer_kernel<NN, true><<<grid, block, 0, stream>>>(G, B, dA, mask, M, (int)N, K, accumulate != 0) \
-        : q8_outer_kernel<NN, false><<<grid, block, 0, stream>>>(G, B, dA, mask, M, (int)N, K, accumulate != 0))
-  if (N <= 4) MG_OUTER(4);
-  else if (N <= 8) MG_OUTER(8);
-  else if (N <= 12) MG_OUTER(12);
-  else MG_OUTER(16);
-#undef MG_OUTER
+  switch ((N + 1) / 2) {
+    case 1: launch_outer<2>(grid, block, pair, access, G, B, dA, mask, M, (int)N, K, accumulate != 0); break;
+    case 2: launch_outer<4>(grid, block, pair, access, G, B, dA, mask, M, (int)N, K, accumulate != 0); break;
+    case 3: launch_outer<6>(grid, block, pair, access, G, B, dA, mask, M, (int)N, K, accumulate != 0); break;
+    case 4: launch_outer<8>(grid, block, pair, access, G, B, dA, mask, M, (int)N, K, accumulate != 0); break;
+    case 5: launch_outer<10>(grid, block, pair, access, G, B, dA, mask, M, (int)N, K, accumulate != 0); break;
+    case 6: launch_outer<12>(grid, block, pair, access, G, B, dA, mask, M, (int)N, K, accumulate != 0); break;
+    case 7: launch_outer<14>(grid, block, pair, access, G, B, dA, mask, M, (int)N, K, accumulate != 0); break;
+    default: launch_outer<16>(grid, block, pair, access, G, B, dA, mask, M, (int)N, K, accumulate != 0); break;
+  }
   MG_LAUNCH_CHECK("gemm_nt_q8 (few columns)");
   return MG_OK;
 }
+
+// dB[K][N] (+)= (codes scales)[M][K]^T . G[M][N], N <= 32.  A CTA takes one block of 64
+// columns of the codes (so one scale per row) and a piece of the rows; its four warps
+// take every fourth row, a lane two columns with their N sums each.  The warps' sums are
+// added up in order, the pieces' by a second kernel, in order.  Bound by the fp64 units:
+// N + 2 instructions per code.
+constexpr int kTallThreads = 128, kTallRows = 32;
+
+template <int NN, int ACCESS>
+__global__ void __launch_bounds__(kTallThreads, NN <= 12 ? 6 : (NN <= 16 ? 5 : 3))
+q8_tall_kernel(const signed char *__restrict__ codes, const double *__restrict__ scales,
+               const double *__restrict__ G, double *__restrict__ parts, size_t M, int N, size_t K, size_t nb,
+               size_t piece) {
+  // gs is reused for the sums: NN x 64 doubles fit kRing x 32 x NN.
+  __shared__ __align__(16) double gs[kRing][kTallRows * NN];
+  __shared__ __align__(16) double ss[kRing][kTallRows];
+  __shared__ __align__(16) uint8_t cs[kRing][kTallRows * 64];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const size_t col0 = (size_t)blockIdx.x * 64, begin = blockIdx.y * piece, end = begin + piece < M ? begin + piece : M;
+  if (N < NN)
+    for (int i = threadIdx.x; i < kRing * kTallRows * (NN - N); i += kTallThreads) {
+      const int s = i / (kTallRows * (NN - N)), j = i - s * kTallRows * (NN - N);
+      gs[s][(j / (NN - N)) * NN + N + j % (NN - N)] = 0.0;
+    }
+  const bool run = N == NN && (reinterpret_cast<uintptr_t>(G) & 15) == 0;
+  auto fetch = [&](size_t m0, int stage) {
+    if (m0 < end) {
+      const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 16;
+      copy_codes<ACCESS>(&cs[stage][r * 64 + c], codes, m0 + r, end, col0 + c, K);
+      if (threadIdx.x < kTallRows) {
+        const bool in = m0 + threadIdx.x < end;
+        copy8(&ss[stage][threadIdx.x], in ? scales + (m0 + threadIdx.x) * nb + blockIdx.x : scales, in);
+      }
+      copy_g<NN>(gs[stage], G, m0, end, kTallRows, N, threadIdx.x, kTallThreads, run);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  double a0[NN], a1[NN];
+#pragma unroll
+  for (int n = 0; n < NN; n++) a0[n] = a1[n] = 0.0;
+#pragma unroll
+  for (int s = 0; s < kRing - 1; s++) fetch(begin + s * kTallRows, s);
+  int stage = 0;
+  for (size_t m0 = begin; m0 < end; m0 += kTallRows) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
+    __syncthreads();  // the stage is complete, and the one before it is read no more
+    fetch(m0 + (kRing - 1) * kTallRows, stage == 0 ? kRing - 1 : stage - 1);
+#pragma unroll 2
+    for (int r = warp; r < kTallRows; r += 4) {  // (rows behind the end are zeros)
+      const int two = *reinterpret_cast<const unsigned short *>(&cs[stage][r * 64 + 2 * lane]) ^ 0x8080;
+      const double s = ss[stage][r];
+      // the byte, its top bit flipped, as the low end of 2^52 + byte + 128
+      const double x0 = (__hiloint2double(0x43300000, two & 255) - 4503599627370624.0) * s;
+      const double x1 = (__hiloint2double(0x43300000, two >> 8) - 4503599627370624.0) * s;
+      const double *g = &gs[stage][r * NN];
+#pragma unroll
+      for (int n = 0; n < NN; n += 2) {
+        const double2 v = *reinterpret_cast<const double2 *>(g + n);
+        a0[n] = fma(x0, v.x, a0[n]);
+        a1[n] = fma(x1, v.x, a1[n]);
+        a0[n + 1] = fma(x0, v.y, a0[n + 1]);
+        a1[n + 1] = fma(x1, v.y, a1[n + 1]);
+      }
+    }
+    stage = stage + 1 == kRing ? 0 : stage + 1;
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  double *sums = &gs[0][0];  // [n][column]
+  for (int w = 0; w < 4; w++) {
+    __syncthreads();
+    if (warp == w) {
+#pragma unroll
+      for (int n = 0; n < NN; n++) {
+        double2 *s = reinterpret_cast<double2 *>(sums + n * 64 + 2 * lane);
+        const double2 o = w == 0 ? make_double2(0.0, 0.0) : *s;
+        *s = make_double2(o.x + a0[n], o.y + a1[n]);
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 64 * N; i += kTallThreads) {
+    const int c = i / N, n = i - c * N;
+    if (col0 + c < K) parts[(blockIdx.y * K + col0 + c) * N + n] = sums[n * 64 + c];
+  }
+}
+
+__global__ void __launch_bounds__(256)
+q8_tall_join_kernel(const double *__restrict__ parts, size_t pieces, size_t n, double *dB, bool accumulate) {
+  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  double s = 0.0;
+#pragma unroll 8
+  for (size_t k = 0; k < pieces; k++) s += __ldcs(parts + k * n + i);
+  dB[i] = accumulate ? dB[i] + s : s;
+}
+
+template <int NN>
+static int launch_tall(const signed char *codes, const double *scales, const double *G, double *dB, size_t M, size_t N,
+                       size_t K, int accumulate) {
+  Context &c = ctx();
+  const size_t gx = q8_blocks(K);
+  // One wave, each CTA with at least four tiles of rows.
+  size_t pieces = (size_t)c.sm_count * (NN <= 12 ? 6 : (NN <= 16 ? 5 : 3)) / gx;
+  if (pieces < 1) pieces = 1;
+  const size_t most = (M + 4 * kTallRows - 1) / (4 * kTallRows);
+  if (pieces > most) pieces = most;
+  const size_t piece = ((M + pieces - 1) / pieces + kTallRows - 1) / kTallRows * kTallRows;
+  pieces = (M + piece - 1) / piece;
+  double *parts = dB;
+  const bool direct = pieces == 1 && !accumulate;
+  if (!direct) {
+    int rc = mg_alloc(pieces * K * N, &parts);
+    if (rc != MG_OK) return rc;
+  }
+  const dim3 grid((unsigned)gx, (unsigned)pieces);
+  const int access = code_access(codes, K);
+  if (access == kCodes16)
+    q8_tall_kernel<NN, kCodes16><<<grid, kTallThreads, 0, c.stream>>>(codes, scales, G, parts, M, (int)N, K, gx, piece);
+  else if (access == kCodes4)
+    q8_tall_kernel<NN, kCodes4><<<grid, kTallThreads, 0, c.stream>>>(codes, scales, G, parts, M, (int)N, K, gx, piece);
+  else
+    q8_tall_kernel<NN, kCodes1><<<grid, kTallThreads, 0, c.stream>>>(codes, scales, G, parts, M, (int)N, K, gx, piece);
+  MG_LAUNCH_CHECK("gemm_tn_q8 (few columns)");
+  if (direct) return MG_OK;
+  q8_tall_join_kernel<<<(unsigned)((K * N + 255) / 256), 256, 0, c.stream>>>(parts, pieces, K * N, dB, accumulate != 0);
+  MG_LAUNCH_CHECK("gemm_tn_q8 (join)");
+  return mg_free(parts);
+}
+
+static int tall_q8(const signed char *codes, const double *scales, const double *G, double *dB, size_t M, size_t N,
+                   size_t K, int accumulate) {
+  if (N <= 2) return launch_tall<2>(codes, scales, G, dB, M, N, K, accumulate);
+  if (N <= 4) return launch_tall<4>(codes, scales, G, dB, M, N, K, accumulate);
+  if (N <= 6) return launch_tall<6>(codes, scales, G, dB, M, N, K, accumulate);
+  if (N <= 8) return launch_tall<8>(codes, scales, G, dB, M, N, K, accumulate);
+  if (N <= 10) return launch_tall<10>(codes, scales, G, dB, M, N, K, accumulate);
+  if (N <= 12) return launch_tall<12>(codes, scales, G, dB, M, N, K, accumulate);
+  if (N <= 16) return launch_tall<16>(codes, scales, G, dB, M, N, K, accumulate);
+  if (N <= 24) return launch_tall<24>(codes, scales, G, dB, M, N, K, accumulate);
+  return launch_tall<32>(codes, scales, G, dB, M, N, K, accumulate);
+}
+
+// x[M][pitch] = the values of codes[M][N]; what is behind the N columns stays as it is.
+static int unpack_rows(const signed char *codes, const double *scales, double *x, size_t pitch, size_t M, size_t N) {
+  const size_t nb = q8_blocks(N), blocks = M * nb;
+  cudaStream_t stream = ctx().stream;
+  int vec = q8_vec(x, codes, N);
+  if (pitch % 4 != 0 && vec == 4) vec = pitch % 2 == 0 ? 2 : 1;
+  const unsigned grid = grid_for(blocks * (vec == 4 ? 16 : 32), kQ8Threads, 64);
+  if (vec == 4 && N % 64 == 0 && pitch == N)
+    q8_unpack_kernel<4, 4, true><<<grid, kQ8Threads, 0, stream>>>(codes, scales, x, pitch, blocks, N, (unsigned)nb);
+  else if (vec == 4)
+    q8_unpack_kernel<4, 2, false><<<grid, kQ8Threads, 0, stream>>>(codes, scales, x, pitch, blocks, N, (unsigned)nb);
+  else if (vec == 2)
+    q8_unpack_kernel<2, 4, false><<<grid, kQ8Threads, 0, stream>>>(codes, scales, x, pitch, blocks, N, (unsigned)nb);
+  else
+    q8_unpack_kernel<1, 4, false><<<grid, kQ8Threads, 0, stream>>>(codes, scales, x, pitch, blocks, N, (unsigned)nb);
+  MG_LAUNCH_CHECK("q8_unpack");
+  return MG_OK;
+}
+
+// fp64 values held at a time for a weight gradient.
+constexpr size_t kQ8UnpackBytes = (size_t)256 << 20;
 
 static int check_q8(const char *name, size_t M, size_t N) {
   if (M >= ((size_t)1 << 40) || N >= ((size_t)1 << 36) || (M && N > ((size_t)1 << 60) / M))
@@ -391,20 +613,7 @@ int mg_q8_unpack(const signed char *codes, const double *scales, double *x, size
   if (M && N && (!x || !codes || !scales)) return fail(MG_ERR_INVALID, "mg_q8_unpack: null pointer");
   MG_ENSURE_INIT();
   if (M == 0 || N == 0) return MG_OK;
-  const size_t nb = q8_blocks(N), blocks = M * nb;
-  cudaStream_t stream = ctx().stream;
-  const int vec = q8_vec(x, codes, N);
-  const unsigned grid = grid_for(blocks * (vec == 4 ? 16 : 32), kQ8Threads, 64);
-  if (vec == 4 && N % 64 == 0)
-    q8_unpack_kernel<4, 4, true><<<grid, kQ8Threads, 0, stream>>>(codes, scales, x, blocks, N, (unsigned)nb);
-  else if (vec == 4)
-    q8_unpack_kernel<4, 2, false><<<grid, kQ8Threads, 0, stream>>>(codes, scales, x, blocks, N, (unsigned)nb);
-  else if (vec == 2)
-    q8_unpack_kernel<2, 4, false><<<grid, kQ8Threads, 0, stream>>>(codes, scales, x, blocks, N, (unsigned)nb);
-  else
-    q8_unpack_kernel<1, 4, false><<<grid, kQ8Threads, 0, stream>>>(codes, scales, x, blocks, N, (unsigned)nb);
-  MG_LAUNCH_CHECK("q8_unpack");
-  return MG_OK;
+  return unpack_rows(codes, scales, x, N, M, N);
 }
 
 int mg_relu_bwd_q8(const signed char *codes, const double *g, double *gx, size_t n, int flags) {
@@ -425,31 +634,34 @@ int mg_gemm_tn_q8(const signed char *codes, const double *scales, const double *
     return fail(MG_ERR_INVALID, "mg_gemm_tn_q8: null pointer");
   MG_ENSURE_INIT();
   if (K == 0 || N == 0) return MG_OK;
-  // Output [K][N], contraction over the M rows; the codes are widened inside the kernel.
-  // Rows of codes or of G that it cannot take are copied into rows that it can.
-  GemmExt e{{nullptr, G, dB, K, N, M, false, false, accumulate, MG_EPI_NONE, nullptr}};
-  e.codes = codes;
-  e.scales = scales;
-  e.lda = K;
-  const bool copy_codes = K % 16 != 0 || off_16_bytes(codes), copy_g = N % 2 != 0 || off_16_bytes(G);
-  if (!copy_codes && !copy_g) return run_gemm_ext(e);
-  const size_t pitch_c = pitch16(K), pitch_g = pitch16(N);
-  const size_t code_room = copy_codes ? (M * pitch_c + 255) / 256 * 32 : 0;  // in doubles
+  if (M == 0) return accumulate ? MG_OK : mg_fill(dB, 0.0, K * N);
+  if (N <= 32) return tall_q8(codes, scales, G, dB, M, N, K, accumulate);
+  // Output [K][N], contraction over the M rows: the tensor kernel on the fp64 form of as
+  // many rows at a time as kQ8UnpackBytes hold.  Widening costs 9 bytes of traffic per
+  // code against 2 N flop: 2 % of the product at 1024 columns.  (Codes widened by the
+  // kernel's own producer warps were slower: the fp64 units, or the warps' latency, then
+  // hold up the tensor instructions; 4.32 ms against 4.05 at 65 536 x 1024 x 1024.)
+  const size_t pitch = pitch16(K), pitch_g = pitch16(N);
+  const bool copy_g = N % 2 != 0 || off_16_bytes(G);
+  size_t rows = kQ8UnpackBytes / 8 / pitch / 64 * 64;
+  if (rows < 64) rows = 64;
+  if (rows > M) rows = M;
   double *room = nullptr;
-  rc = mg_alloc(code_room + (copy_g ? M * pitch_g : 0), &room);
+  rc = mg_alloc(rows * pitch + (copy_g ? rows * pitch_g : 0), &room);
   if (rc != MG_OK) return rc;
-  if (copy_codes) {
-    signed char *dst = reinterpret_cast<signed char *>(room);
-    rc = copy_codes_rows(codes, M, K, dst, pitch_c);
-    e.codes = dst;
-    e.lda = pitch_c;
+  const size_t nb = q8_blocks(K);
+  for (size_t m = 0; m < M && rc == MG_OK; m += rows) {
+    const size_t part = M - m < rows ? M - m : rows;
+    rc = unpack_rows(codes + m * K, scales + m * nb, room, pitch, part, K);
+    GemmExt e{{room, G + m * N, dB, K, N, part, false, false, accumulate || m > 0, MG_EPI_NONE, nullptr}};
+    e.lda = pitch;
+    if (rc == MG_OK && copy_g) {
+      e.d.B = room + rows * pitch;
+      e.ldb = pitch_g;
+      rc = copy_rows(G + m * N, part, N, N, room + rows * pitch, pitch_g);
+    }
+    if (rc == MG_OK) rc = run_gemm_ext(e);
   }
-  if (rc == MG_OK && copy_g) {
-    rc = copy_rows(G, M, N, N, room + code_room, pitch_g);
-    e.d.B = room + code_room;
-    e.ldb = pitch_g;
-  }
-  if (rc == MG_OK) rc = run_gemm_ext(e);
   const int freed = mg_free(room);
   return rc != MG_OK ? rc : freed;
 }
