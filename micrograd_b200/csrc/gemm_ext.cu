@@ -117,12 +117,14 @@ int run_gemm_ext(const GemmExt &e) {
     MG_LAUNCH_CHECK("gemm (empty contraction)");
     return MG_OK;
   }
-  if (!e.mask8 && dense && (d.M > 64 || d.N <= (size_t)SkinnyCfg::BN)) return run_gemm(d);
-  if ((lda & 1) || off_16_bytes(d.A) || (ldb & 1) || off_16_bytes(d.B))
-    return fail(MG_ERR_INVALID, "gemm: operand rows do not start on 16-byte boundaries");
   Context &c = ctx();
   const int M = (int)d.M, N = (int)d.N, K = (int)d.K;
   const GemmPlan plan = plan_ext(M, N, K, c.sm_count);
+  const int tiles_m = (M + plan.bm - 1) / plan.bm, tiles_n = (N + plan.bn - 1) / plan.bn;
+  const bool fold_here = plan.spans >= kFoldBySegments * tiles_m * tiles_n;
+  if (!e.mask8 && dense && !fold_here && (d.M > 64 || d.N <= (size_t)SkinnyCfg::BN)) return run_gemm(d);
+  if ((lda & 1) || off_16_bytes(d.A) || (ldb & 1) || off_16_bytes(d.B))
+    return fail(MG_ERR_INVALID, "gemm: operand rows do not start on 16-byte boundaries");
   DmmaLaunch L{};
   bool ok_a, ok_b;
   if (d.a_kcontig) {
@@ -153,7 +155,6 @@ int run_gemm_ext(const GemmExt &e) {
   ep.mask8 = e.mask8;
   ep.ld_mask8 = d.N;
   ep.pairs = ldd % 2 == 0 && !off_16_bytes(d.D) && !(reinterpret_cast<uintptr_t>(e.mask8) & 1);
-  const int tiles_m = (M + plan.bm - 1) / plan.bm, tiles_n = (N + plan.bn - 1) / plan.bn;
   const int KT = (K + BK - 1) / BK;
   const SegTable *table = nullptr;
   if (plan.spans > 0) {
@@ -170,7 +171,7 @@ int run_gemm_ext(const GemmExt &e) {
   L.M = M; L.N = N; L.K = K;
   L.tiles_m = tiles_m; L.tiles_n = tiles_n;
   L.table = table ? table->dev_items : nullptr;
-  const bool split = table && table->slots > 0, fold_here = split && plan.spans >= kFoldBySegments * tiles_m * tiles_n;
+  const bool split = table && table->slots > 0;
   L.tickets = split && !fold_here ? table->dev_tickets : nullptr;
   L.items = table ? table->items : tiles_m * tiles_n;
   L.min_nkt = table ? table->min_nkt : KT;
@@ -178,7 +179,7 @@ int run_gemm_ext(const GemmExt &e) {
   if (d.a_kcontig && !d.b_kcontig) rc = launch_layout_ext<true, false>(plan.tile, L);
   else if (d.a_kcontig) rc = launch_layout_ext<true, true>(plan.tile, L);
   else rc = launch_layout_ext<false, false>(plan.tile, L);
-  if (rc != MG_OK || !fold_here) return rc;
+  if (rc != MG_OK || !split || !fold_here) return rc;
   fold_tiles_kernel<<<dim3((unsigned)((plan.bm * plan.bn + 255) / 256), (unsigned)(tiles_m * tiles_n)), 256, 0,
                       c.stream>>>(ep, table->dev_tiles, tiles_n, plan.bm, plan.bn, M, N);
   MG_LAUNCH_CHECK("gemm fold");

@@ -288,11 +288,14 @@ __device__ __forceinline__ void copy_codes(uint8_t *dst, const signed char *__re
 // output, 9 bytes per element (17 when accumulating).  TX x TY threads take 2 TX columns
 // of 8 TY rows at a time.  PAIR: the two columns of a thread are neighbours (K even,
 // dA aligned), else TX apart.
+// Two CTAs per SM with more than eight columns: 108 us for 65 536 x 1024, ten columns;
+// three spill registers, 122 us.
+constexpr int outer_ctas(int nn) { return nn <= 8 ? 4 : 2; }
 constexpr int kOuterRows = 8;  // rows per thread and tile
 constexpr int kOuterCodes = 256 * 2 * kOuterRows;  // codes of a tile
 
 template <int NN, bool PAIR, int ACCESS>
-__global__ void __launch_bounds__(256, NN <= 8 ? 4 : 3)
+__global__ void __launch_bounds__(256, outer_ctas(NN))
 q8_outer_kernel(const double *__restrict__ G, const double *__restrict__ B, double *dA,
                 const signed char *__restrict__ mask, size_t M, int N, size_t K, bool accumulate) {
   constexpr int kMostRows = kOuterRows * 8;
@@ -392,7 +395,7 @@ static int outer_q8(const double *G, const double *B, double *dA, size_t M, size
   const int access = code_access(mask, K);
   const size_t rows = (size_t)kOuterRows * (256 / tx), gx = (K + 2 * tx - 1) / (2 * tx), tiles = (M + rows - 1) / rows;
   // (one wave: a CTA's start, its rows of B, costs as much as several tiles)
-  size_t gy = (size_t)ctx().sm_count * (N <= 8 ? 4 : 3) / gx;
+  size_t gy = (size_t)ctx().sm_count * outer_ctas((int)N) / gx;
   if (gy < 1) gy = 1;
   if (gy > tiles) gy = tiles;
   const dim3 grid((unsigned)gx, (unsigned)gy), block(tx, 256 / tx);
@@ -416,9 +419,12 @@ static int outer_q8(const double *G, const double *B, double *dA, size_t M, size
 // added up in order, the pieces' by a second kernel, in order.  Bound by the fp64 units:
 // N + 2 instructions per code.
 constexpr int kTallThreads = 128, kTallRows = 32;
+// CTAs per SM: 65 536 x 1024, ten columns: 98 us with four and all eight rows of a warp
+// unrolled, 112 with six and two rows (more warps, but twice the instructions a row).
+constexpr int tall_ctas(int nn) { return nn <= 16 ? 4 : 3; }
 
 template <int NN, int ACCESS>
-__global__ void __launch_bounds__(kTallThreads, NN <= 12 ? 6 : (NN <= 16 ? 5 : 3))
+__global__ void __launch_bounds__(kTallThreads, tall_ctas(NN))
 q8_tall_kernel(const signed char *__restrict__ codes, const double *__restrict__ scales,
                const double *__restrict__ G, double *__restrict__ parts, size_t M, int N, size_t K, size_t nb,
                size_t piece) {
@@ -456,8 +462,9 @@ q8_tall_kernel(const signed char *__restrict__ codes, const double *__restrict__
     asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
     __syncthreads();  // the stage is complete, and the one before it is read no more
     fetch(m0 + (kRing - 1) * kTallRows, stage == 0 ? kRing - 1 : stage - 1);
-#pragma unroll 2
-    for (int r = warp; r < kTallRows; r += 4) {  // (rows behind the end are zeros)
+#pragma unroll
+    for (int r0 = 0; r0 < kTallRows; r0 += 4) {  // (rows behind the end are zeros)
+      const int r = r0 + warp;
       const int two = *reinterpret_cast<const unsigned short *>(&cs[stage][r * 64 + 2 * lane]) ^ 0x8080;
       const double s = ss[stage][r];
       // the byte, its top bit flipped, as the low end of 2^52 + byte + 128
@@ -511,7 +518,7 @@ static int launch_tall(const signed char *codes, const double *scales, const dou
   Context &c = ctx();
   const size_t gx = q8_blocks(K);
   // One wave, each CTA with at least four tiles of rows.
-  size_t pieces = (size_t)c.sm_count * (NN <= 12 ? 6 : (NN <= 16 ? 5 : 3)) / gx;
+  size_t pieces = (size_t)c.sm_count * tall_ctas(NN) / gx;
   if (pieces < 1) pieces = 1;
   const size_t most = (M + 4 * kTallRows - 1) / (4 * kTallRows);
   if (pieces > most) pieces = most;
