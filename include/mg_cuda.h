@@ -185,6 +185,8 @@ int mg_colsum_noalloc(const double *g, double *out_row, size_t M, size_t N, int 
  * result does not depend on the run. */
 int mg_sum_all_fwd(const double *x, double *out1, size_t n);
 int mg_sum_all_bwd(const double *g1, double *gx, size_t n, int flags);
+/* y[n] += a1[0] * x[n], the factor read on the device (MG_ACC_STORE_A: y = ...). */
+int mg_scale_acc(const double *a1, const double *x, double *y, size_t n, int flags);
 /* Last-axis sum [M,N] -> [M] (no counterpart in the reference). */
 int mg_sum_lastaxis_fwd(const double *x, double *out, size_t M, size_t N);
 int mg_sum_lastaxis_bwd(const double *g, double *gx, size_t M, size_t N, int flags);
@@ -319,6 +321,7 @@ int mg_sgd_step_multi(double *const *params, const double *const *grads, const s
  * replays, so results can be read (mg_download) after every mg_graph_launch(). */
 int mg_graph_begin(void);
 int mg_graph_end(int *out_id);
+int mg_graph_recording(void); /* 1 between mg_graph_begin() and mg_graph_end() */
 int mg_graph_launch(int id);  /* enqueues the whole recorded step on the compute stream */
 int mg_graph_kernels(int id); /* kernel launches the recorded step contains (0 if unknown id) */
 int mg_graph_destroy(int id);

@@ -30,6 +30,7 @@ extern "C" {
 typedef struct mgt_tensor_s *mgt_tensor; /* owns one std::shared_ptr<Tensor>   */
 typedef struct mgt_linear_s *mgt_linear; /* owns one Linear                    */
 typedef struct mgt_sgd_s *mgt_sgd;       /* owns one SGD                       */
+typedef struct mgt_norm_s *mgt_norm;     /* owns one GroupNorm (extension)     */
 
 const char *mgt_last_error(void);
 
@@ -101,6 +102,20 @@ int mgt_comm_world(void);
 int mgt_argmax_rows(mgt_tensor x, int *out, size_t nrows);
 mgt_tensor mgt_linear_forward_relu(mgt_linear l, mgt_tensor input);
 int mgt_set_requires_grad(mgt_tensor t, int flag);
+/* linear_cross_entropy: the layer's softmax cross-entropy without its logits.
+ * denom: divisor of the mean; 0 = number of rows.  Label -1: row left out. */
+mgt_tensor mgt_linear_cross_entropy(mgt_tensor input, mgt_linear head, mgt_tensor labels, double denom);
+mgt_tensor mgt_linear_cross_entropy_host(mgt_tensor input, mgt_linear head, const int *labels_host,
+                                         size_t nrows, double denom);
+/* GroupNorm; activation: 0 none, 1 ReLU, 2 SiLU */
+mgt_norm mgt_norm_new(size_t groups, size_t channels, double eps);
+void mgt_norm_release(mgt_norm n);
+mgt_tensor mgt_norm_forward(mgt_norm n, mgt_tensor input, int activation);
+mgt_tensor mgt_norm_weights(mgt_norm n);
+mgt_tensor mgt_norm_bias(mgt_norm n);
+/* Tensor::keep_8bit and whether it is in force */
+int mgt_keep_8bit(mgt_tensor t);
+int mgt_kept_8bit(mgt_tensor t);
 int mgt_sync(void);
 /* data-parallel training */
 int mgt_comm_unique_id(char *out128);

@@ -93,6 +93,22 @@ public:
   // `values` must stay unchanged until that next use has completed (pinned memory
   // for a copy that really overlaps).  Not for the input of a recorded step.
   void prefetch_from_host(const double *values);
+  // Keeps the values in 8 bits from now on, about a seventh of the memory: a code per
+  // value and a scale per 64 columns of the last axis, within half a step of 1/127 of
+  // each block's largest magnitude (and never 0 for a value that is not).  Meant for
+  // activations between their last use in the forward pass and the backward pass:
+  //
+  //   auto h = l1.forward_relu(x), logits = l2.forward(h);
+  //   h->keep_8bit();
+  //
+  // The tensor's values ARE those the codes stand for afterwards.  The weight gradient
+  // of a Linear or matmul, and ReLU masks (which stay exact: a code has the sign of its
+  // value), read the codes themselves; any other use makes an fp64 form of them again,
+  // any write to the tensor ends the 8-bit form.  Refused (std::logic_error) for tensors
+  // whose values share a buffer (parameters after SGD::enable_allreduce, load_mnist
+  // samples), and, while a step is recorded, for tensors made before the recording.
+  void keep_8bit();
+  bool kept_8bit() const;
   // Read-only host views.  Unlike the mutable data()/grad() of the reference
   // interface they do not hand out a writable reference, so the device copy stays
   // current and no re-upload follows the read.

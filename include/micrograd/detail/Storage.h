@@ -69,6 +69,14 @@ public:
   // Uses caller-owned device memory that already holds the values (a slice of a
   // larger upload); `keepalive` owns that memory.
   void adopt(double *slice, std::shared_ptr<void> keepalive);
+  // Keeps the contents in 8 bits from now on (rows x cols = size()): codes and a scale
+  // per 64 columns, as mg_q8_pack makes them; the fp64 buffer is given up.  The contents
+  // ARE the values the codes stand for from here on.  device_read() makes an fp64 buffer
+  // of them again (the codes stay), any write drops the codes.
+  void pack8(size_t rows, size_t cols);
+  bool packed() const { return codes_ != nullptr; }
+  const signed char *codes() const { return codes_; }
+  const double *scales() const { return scales_; }
   // True when the device buffer holds the current values (not logical zeros,
   // not superseded by a lent host view).
   bool device_current() const { return !zero_ && dev_valid_; }
@@ -85,6 +93,9 @@ private:
   void settle_exchange();  // make the compute stream wait for a pending all-reduce
   void sync_device_from_host();
   void sync_host_from_device();
+  void drop_codes();     // the contents are about to be replaced
+  void expand();         // dev_ from the codes
+  void download(double *values, size_t first, size_t n);  // current device contents, from either form
   bool fetch_mirror(double *value);  // true: *value is the mirrored, still current element
 
   size_t size_ = 0;
@@ -100,6 +111,11 @@ private:
   int pending_upload_ = -1;  // event id of a prefetch the compute stream has not waited for
   unsigned long long mirror_ticket_ = 0;  // pending scalar mirror (0: none)
   unsigned long long mirror_stamp_ = 0;   // write_stamp_ when the mirror was started
+  signed char *codes_ = nullptr;  // 8-bit form of the contents (with scales_), or null
+  double *scales_ = nullptr;
+  size_t code_rows_ = 0, code_cols_ = 0;
+  bool dev_recorded_ = false;     // dev_ was allocated while a step was being recorded
+  bool codes_recorded_ = false;
   std::vector<double> host_;
 };
 

@@ -35,6 +35,30 @@ private:
   std::shared_ptr<Tensor> bias_;
 };
 
+namespace micrograd {
+enum class Activation { None, ReLU, SiLU };  // SiLU: z / (1 + exp(-z))
+}
+
+// addition: group norm with an activation, channels last.  forward([N, ..., channels])
+// normalises, for each of the N samples, the values of every group of channels /
+// groups neighbouring channels over all positions between (none for [N, channels]) to
+// mean 0 and variance 1 / (1 + eps / variance), scales and shifts each channel by
+// weights() (1 at first) and bias() (0), and applies the activation, as one node.
+class GroupNorm {
+public:
+  GroupNorm(size_t groups, size_t channels, double eps = 1e-5);
+  std::shared_ptr<Tensor> forward(const std::shared_ptr<Tensor> &input,
+                                  micrograd::Activation activation = micrograd::Activation::None);
+  std::shared_ptr<Tensor> weights();
+  std::shared_ptr<Tensor> bias();
+
+private:
+  size_t groups_, channels_;
+  double eps_;
+  std::shared_ptr<Tensor> weights_;
+  std::shared_ptr<Tensor> bias_;
+};
+
 class SGD {
 public:
   SGD(std::vector<std::shared_ptr<Tensor>> parameters, double learning_rate);
@@ -82,5 +106,17 @@ std::shared_ptr<Tensor> softmax_cross_entropy(const std::shared_ptr<Tensor> &log
                                               double denom = 0.0);
 std::shared_ptr<Tensor> softmax_cross_entropy(const std::shared_ptr<Tensor> &logits,
                                               const std::vector<int> &labels, double denom = 0.0);
+// The same loss of head.forward(input) for heads with many classes, without the [B, C]
+// logits: they exist for a block of rows at a time (at most 1 GiB).  The gradients are
+// computed in the forward pass, which has the block's logits at hand (three products
+// instead of the four that going through them again in the backward pass would take),
+// and kept for backward(); where neither the input nor the head's parameters require a
+// gradient only the loss is computed.  A row with label -1 is left out (a padded
+// batch): it adds nothing to the loss or any gradient, whatever its values are; it does
+// count in the default divisor.
+std::shared_ptr<Tensor> linear_cross_entropy(const std::shared_ptr<Tensor> &input, Linear &head,
+                                             const std::shared_ptr<Tensor> &labels, double denom = 0.0);
+std::shared_ptr<Tensor> linear_cross_entropy(const std::shared_ptr<Tensor> &input, Linear &head,
+                                             const std::vector<int> &labels, double denom = 0.0);
 // Index of the first strict maximum of each row of a 2-D tensor.
 std::vector<int> argmax_rows(const std::shared_ptr<Tensor> &x);

@@ -69,6 +69,7 @@ SIGNATURES = {
     "mg_colsum_noalloc": (C.c_int, [C.c_void_p, C.c_void_p, _sz, _sz, C.c_int]),
     "mg_sum_all_fwd": (C.c_int, [C.c_void_p, C.c_void_p, _sz]),
     "mg_sum_all_bwd": (C.c_int, [C.c_void_p, C.c_void_p, _sz, C.c_int]),
+    "mg_scale_acc": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, _sz, C.c_int]),
     "mg_sum_lastaxis_fwd": (C.c_int, [C.c_void_p, C.c_void_p, _sz, _sz]),
     "mg_sum_lastaxis_bwd": (C.c_int, [C.c_void_p, C.c_void_p, _sz, _sz, C.c_int]),
     "mg_gemm_nn": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, _sz, _sz, _sz, C.c_int, C.c_int,
@@ -95,6 +96,7 @@ SIGNATURES = {
     "mg_sgd_step": (C.c_int, [C.c_void_p, C.c_void_p, C.c_double, _sz]),
     "mg_graph_begin": (C.c_int, []),
     "mg_graph_end": (C.c_int, [_ip]),
+    "mg_graph_recording": (C.c_int, []),
     "mg_graph_launch": (C.c_int, [C.c_int]),
     "mg_graph_kernels": (C.c_int, [C.c_int]),
     "mg_graph_destroy": (C.c_int, [C.c_int]),
@@ -131,7 +133,7 @@ SIGNATURES = {
 
 # Entry points whose int result is a value, not a status.
 _VALUE_INT = {"mg_device", "mg_sm_count", "mg_comm_rank", "mg_comm_world", "mg_comm_peer_path",
-              "mg_graph_kernels"}
+              "mg_graph_kernels", "mg_graph_recording"}
 
 
 def declared_in_header(header_text: str) -> list[str]:

@@ -555,6 +555,8 @@ int mg_graph_end(int *out_id) {
   return MG_OK;
 }
 
+int mg_graph_recording(void) { return g_ctx.capturing ? 1 : 0; }
+
 int mg_graph_launch(int id) {
   MG_ENSURE_INIT();
   MG_NOT_WHILE_RECORDING("mg_graph_launch");

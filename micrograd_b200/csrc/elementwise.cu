@@ -371,6 +371,17 @@ add_row_kernel(const double *x, const double *__restrict__ row, double *out, siz
 
 // sum() backward: gx[i] += g[0], the scalar read from device memory
 // (src/ops/Reduction.cpp:26-30).  in: old gx.  out: gx.
+// y (+)= a1[0] * x, the factor read on the device.
+struct ScaleAcc {
+  static constexpr int NI = 2, NO = 1;
+  const double *in[2];
+  double *out[1];
+  const double *a1;
+  __device__ __forceinline__ void compute(const double (&i)[2], double (&o)[1]) const {
+    o[0] = i[1] + __ldg(a1) * i[0];
+  }
+};
+
 struct ScalarBroadcastBwd {
   static constexpr int NI = 1, NO = 1;
   const double *in[NI];
@@ -704,6 +715,18 @@ int mg_sum_all_bwd(const double *g1, double *gx, size_t n, int flags) {
   f.out[0] = gx;
   f.g0 = g1;
   return launch_map(f, n, "sum_all_bwd");
+}
+
+int mg_scale_acc(const double *a1, const double *x, double *y, size_t n, int flags) {
+  if (n && (!a1 || !x || !y)) return fail(MG_ERR_INVALID, "mg_scale_acc: null pointer");
+  MG_ENSURE_INIT();
+  if (n == 0) return MG_OK;
+  ScaleAcc f;
+  f.in[0] = x;
+  f.in[1] = (flags & MG_ACC_STORE_A) ? nullptr : y;
+  f.out[0] = y;
+  f.a1 = a1;
+  return launch_map(f, n, "scale_acc");
 }
 
 int mg_sum_lastaxis_bwd(const double *g, double *gx, size_t M, size_t N, int flags) {

@@ -374,6 +374,56 @@ int mgt_argmax_rows(mgt_tensor x, int *out, size_t nrows) {
   });
 }
 
+struct mgt_norm_s {
+  GroupNorm n;
+  mgt_norm_s(size_t g, size_t c, double eps) : n(g, c, eps) {}
+};
+
+mgt_norm mgt_norm_new(size_t groups, size_t channels, double eps) {
+  try {
+    return new mgt_norm_s(groups, channels, eps);
+  } catch (...) {
+    record_current_exception();
+    return nullptr;
+  }
+}
+
+void mgt_norm_release(mgt_norm n) { delete n; }
+
+mgt_tensor mgt_norm_forward(mgt_norm n, mgt_tensor input, int activation) {
+  return guard_tensor([&] {
+    if (activation < 0 || activation > 2) {
+      throw std::invalid_argument("mgt_norm_forward: unknown activation");
+    }
+    return n->n.forward(input->p, static_cast<micrograd::Activation>(activation));
+  });
+}
+
+mgt_tensor mgt_norm_weights(mgt_norm n) {
+  return guard_tensor([&] { return n->n.weights(); });
+}
+
+mgt_tensor mgt_norm_bias(mgt_norm n) {
+  return guard_tensor([&] { return n->n.bias(); });
+}
+
+mgt_tensor mgt_linear_cross_entropy(mgt_tensor input, mgt_linear head, mgt_tensor labels, double denom) {
+  return guard_tensor([&] { return linear_cross_entropy(input->p, head->l, labels->p, denom); });
+}
+
+mgt_tensor mgt_linear_cross_entropy_host(mgt_tensor input, mgt_linear head, const int *labels_host, size_t nrows,
+                                         double denom) {
+  return guard_tensor([&] {
+    return linear_cross_entropy(input->p, head->l, std::vector<int>(labels_host, labels_host + nrows), denom);
+  });
+}
+
+int mgt_keep_8bit(mgt_tensor t) {
+  return guard_int([&] { t->p->keep_8bit(); });
+}
+
+int mgt_kept_8bit(mgt_tensor t) { return t->p->kept_8bit() ? 1 : 0; }
+
 mgt_tensor mgt_linear_forward_relu(mgt_linear l, mgt_tensor input) {
   return guard_tensor([&] { return l->l.forward_relu(input->p); });
 }

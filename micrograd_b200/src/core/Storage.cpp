@@ -37,6 +37,95 @@ Storage::~Storage() {
   if (dev_ && owns_dev_) {
     mg_free(dev_);
   }
+  drop_codes();
+}
+
+void Storage::drop_codes() {
+  if (codes_) {
+    mg_free_i8(codes_);
+    mg_free(scales_);
+    codes_ = nullptr;
+    scales_ = nullptr;
+  }
+}
+
+void Storage::pack8(size_t rows, size_t cols) {
+  if (zero_ || size_ == 0) {
+    return;  // nothing to keep
+  }
+  if (!owns_dev_) {
+    throw std::logic_error("keep_8bit: the values live in a buffer shared with other tensors");
+  }
+  const bool recording = mg_graph_recording() != 0;
+  if (codes_) {
+    // Kept in 8 bits already; an fp64 form that was made of them since goes again.
+    if (dev_ && recording == dev_recorded_) {
+      double *fp64 = dev_;
+      dev_ = nullptr;
+      dev_valid_ = false;
+      check(mg_free(fp64), "free");
+    }
+    return;
+  }
+  device_read();  // settles a pending upload, refreshes the device copy from a lent host view
+  if (recording != dev_recorded_) {
+    throw std::logic_error(recording
+                               ? "keep_8bit: a tensor made before the recording keeps its buffer while a step is recorded"
+                               : "keep_8bit: a tensor made by a recorded step keeps its buffer");
+  }
+  const size_t blocks = (cols + MG_Q8_BLOCK - 1) / MG_Q8_BLOCK;
+  signed char *codes = nullptr;
+  double *scales = nullptr;
+  check(mg_alloc_i8(rows * cols, &codes), "device allocation");
+  int rc = mg_alloc(rows * blocks, &scales);
+  if (rc == MG_OK) {
+    rc = mg_q8_pack(dev_, codes, scales, rows, cols);
+  }
+  if (rc != MG_OK) {
+    mg_free_i8(codes);
+    mg_free(scales);
+    check(rc, "keep_8bit");
+  }
+  write_stamp_++;  // the contents are the codes' values from here on
+  codes_ = codes;
+  scales_ = scales;
+  code_rows_ = rows;
+  code_cols_ = cols;
+  codes_recorded_ = recording;
+  double *fp64 = dev_;
+  dev_ = nullptr;
+  dev_valid_ = false;
+  host_valid_ = false;
+  host_.clear();
+  host_.shrink_to_fit();
+  check(mg_free(fp64), "free");
+}
+
+// An fp64 buffer made while a step is recorded belongs to that step, and one made
+// outside would not follow its replays: codes are expanded on their own side only.
+void Storage::expand() {
+  if ((mg_graph_recording() != 0) != codes_recorded_) {
+    throw std::logic_error("a tensor kept in 8 bits before a recording, or by one, is used on the other side of it");
+  }
+  ensure_device_buffer();
+  check(mg_q8_unpack(codes_, scales_, dev_, code_rows_, code_cols_), "unpack");
+  dev_valid_ = true;
+}
+
+void Storage::download(double *values, size_t first, size_t n) {
+  if (dev_valid_) {
+    check(mg_download(values, dev_ + first, n), "download");
+    return;
+  }
+  // From the codes, whatever side of a recording they were made on.
+  double *fp64 = nullptr;
+  check(mg_alloc(size_, &fp64), "device allocation");
+  int rc = mg_q8_unpack(codes_, scales_, fp64, code_rows_, code_cols_);
+  if (rc == MG_OK) {
+    rc = mg_download(values, fp64 + first, n);
+  }
+  mg_free(fp64);
+  check(rc, "download");
 }
 
 void Storage::init_zero(size_t n) {
@@ -50,6 +139,7 @@ void Storage::ensure_device_buffer() {
   if (!dev_) {
     check(mg_alloc(size_, &dev_), "device allocation");
     owns_dev_ = true;
+    dev_recorded_ = mg_graph_recording() != 0;
   }
 }
 
@@ -90,6 +180,7 @@ void Storage::init_from_pointer(const double *values, size_t n) {
 }
 
 void Storage::sync_device_from_host() {
+  drop_codes();
   ensure_device_buffer();
   check(mg_upload(dev_, host_.data(), size_), "upload");
   dev_valid_ = true;
@@ -111,7 +202,7 @@ void Storage::sync_host_from_device() {
   if (fetch_mirror(&mirrored)) {
     host_[0] = mirrored;
   } else {
-    check(mg_download(host_.data(), dev_, size_), "download");
+    download(host_.data(), 0, size_);
   }
   host_valid_ = true;
   host_epoch_ = g_device_epoch;
@@ -145,6 +236,8 @@ const double *Storage::device_read() {
     zero_ = false;
     dev_valid_ = true;
     host_valid_ = false;
+  } else if (!dev_valid_ && codes_) {
+    expand();
   } else if (!dev_valid_) {
     sync_device_from_host();
   }
@@ -152,6 +245,7 @@ const double *Storage::device_read() {
 }
 
 double *Storage::device_overwrite() {
+  drop_codes();
   write_stamp_++;
   settle_upload();
   ensure_device_buffer();
@@ -164,6 +258,10 @@ double *Storage::device_overwrite() {
 double *Storage::device_accumulate(bool *store) {
   write_stamp_++;
   settle_upload();
+  if (codes_) {
+    device_read();
+    drop_codes();
+  }
   if (zero_) {
     ensure_device_buffer();
     *store = true;
@@ -183,11 +281,13 @@ double *Storage::device_accumulate(bool *store) {
 double *Storage::device_update() {
   write_stamp_++;
   device_read();
+  drop_codes();
   host_valid_ = false;
   return dev_;
 }
 
 void Storage::set_zero() {
+  drop_codes();
   write_stamp_++;
   settle_upload();
   zero_ = true;
@@ -196,6 +296,7 @@ void Storage::set_zero() {
 }
 
 void Storage::fill(double value) {
+  drop_codes();
   write_stamp_++;
   settle_upload();
   ensure_device_buffer();
@@ -214,6 +315,7 @@ std::vector<double> &Storage::host_mutable() {
   write_stamp_++;
   // The caller may write through the reference at any later time, so the host
   // vector is the authority until a kernel needs the values again.
+  drop_codes();
   dev_valid_ = false;
   return host_;
 }
@@ -224,7 +326,7 @@ const std::vector<double> &Storage::host_const() {
     // A read does not end the logical-zero state: the next accumulation is still
     // a plain store and no buffer has to be filled.
     host_.assign(size_, 0.0);
-  } else if (!host_valid_ || (dev_valid_ && host_epoch_ != g_device_epoch)) {
+  } else if (!host_valid_ || ((dev_valid_ || codes_) && host_epoch_ != g_device_epoch)) {
     // (second case: a recorded step was replayed since the host copy was taken)
     sync_host_from_device();
   }
@@ -236,7 +338,7 @@ double Storage::peek(size_t index) {
   if (zero_ || index >= size_) {
     return 0.0;
   }
-  if (host_valid_ && !(dev_valid_ && host_epoch_ != g_device_epoch)) {
+  if (host_valid_ && !((dev_valid_ || codes_) && host_epoch_ != g_device_epoch)) {
     return host_[index];
   }
   double v = 0.0;
@@ -244,11 +346,12 @@ double Storage::peek(size_t index) {
     return v;
   }
   settle_exchange();
-  check(mg_download(&v, dev_ + index, 1), "download");
+  download(&v, index, 1);
   return v;
 }
 
 void Storage::upload_in_place(const double *values) {
+  drop_codes();
   write_stamp_++;
   settle_upload();
   ensure_device_buffer();
@@ -259,6 +362,7 @@ void Storage::upload_in_place(const double *values) {
 }
 
 void Storage::prefetch_in_place(const double *values) {
+  drop_codes();
   write_stamp_++;
   settle_upload();  // an earlier prefetch into the same buffer is ordered first
   ensure_device_buffer();
@@ -273,6 +377,10 @@ void Storage::prefetch_in_place(const double *values) {
 
 void Storage::rehome(double *slice, std::shared_ptr<void> keepalive) {
   settle_upload();
+  if (codes_) {
+    device_read();
+    drop_codes();
+  }
   if (!zero_) {
     if (dev_valid_) {
       check(mg_copy(slice, dev_, size_), "copy");
@@ -290,6 +398,7 @@ void Storage::rehome(double *slice, std::shared_ptr<void> keepalive) {
 }
 
 void Storage::adopt(double *slice, std::shared_ptr<void> keepalive) {
+  drop_codes();
   settle_upload();
   if (dev_ && owns_dev_) {
     check(mg_free(dev_), "free");

@@ -85,6 +85,13 @@ void Tensor::copy_from_host(const double *values) { data_.upload_in_place(values
 
 void Tensor::prefetch_from_host(const double *values) { data_.prefetch_in_place(values); }
 
+void Tensor::keep_8bit() {
+  const size_t cols = shape_.empty() ? 1 : shape_.back();
+  data_.pack8(cols ? data_.size() / cols : 0, cols);
+}
+
+bool Tensor::kept_8bit() const { return data_.packed(); }
+
 const std::vector<double> &Tensor::data() const { return data_.host_const(); }
 
 const std::vector<double> &Tensor::grad() const { return grad_.host_const(); }

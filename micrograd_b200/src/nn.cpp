@@ -111,16 +111,26 @@ std::shared_ptr<Tensor> Linear::fused_forward(const std::shared_ptr<Tensor> &inp
     if (relu && !premasked) {
       // dZ = dOut * (out > 0); out > 0 exactly where the pre-activation was.
       check(mg_alloc(batch * out, &masked), "device allocation");
-      check(mg_unary_bwd(MG_RELU, Access::data(self).device_read(), nullptr, 0.0, g, masked,
-                         batch * out, MG_ACC_STORE_A),
-            "relu mask");
+      if (Access::data(self).packed()) {
+        check(mg_relu_bwd_q8(Access::data(self).codes(), g, masked, batch * out, MG_ACC_STORE_A), "relu mask");
+      } else {
+        check(mg_unary_bwd(MG_RELU, Access::data(self).device_read(), nullptr, 0.0, g, masked,
+                           batch * out, MG_ACC_STORE_A),
+              "relu mask");
+      }
       g = masked;
     }
     bool store = false;
     if (Access::requires_grad(w)) {
       double *gw = Access::grad(w).device_accumulate(&store);
-      check(mg_gemm_tn(Access::data(x).device_read(), g, gw, batch, out, in, store ? 0 : 1),
-            "linear dW");
+      if (Access::data(x).packed()) {
+        check(mg_gemm_tn_q8(Access::data(x).codes(), Access::data(x).scales(), g, gw, batch, out, in,
+                            store ? 0 : 1),
+              "linear dW");
+      } else {
+        check(mg_gemm_tn(Access::data(x).device_read(), g, gw, batch, out, in, store ? 0 : 1),
+              "linear dW");
+      }
     }
     if (Access::requires_grad(b)) {
       double *gb = Access::grad(b).device_accumulate(&store);
@@ -133,10 +143,16 @@ std::shared_ptr<Tensor> Linear::fused_forward(const std::shared_ptr<Tensor> &inp
       const bool mask_input = Access::is_relu_output(x);
       const bool stays_masked = mask_input && Access::grad_fully_masked(x);
       double *gx = Access::grad(x).device_accumulate(&store);
-      check(mg_gemm_nt(g, Access::data(w).device_read(), gx, batch, out, in, store ? 0 : 1,
-                       mask_input ? MG_EPI_RELU_MASK : MG_EPI_NONE,
-                       mask_input ? Access::data(x).device_read() : nullptr),
-            "linear dX");
+      if (mask_input && Access::data(x).packed()) {
+        check(mg_gemm_nt_q8(g, Access::data(w).device_read(), gx, batch, out, in, store ? 0 : 1,
+                            Access::data(x).codes()),
+              "linear dX");
+      } else {
+        check(mg_gemm_nt(g, Access::data(w).device_read(), gx, batch, out, in, store ? 0 : 1,
+                         mask_input ? MG_EPI_RELU_MASK : MG_EPI_NONE,
+                         mask_input ? Access::data(x).device_read() : nullptr),
+              "linear dX");
+      }
       if (mask_input) {
         Access::commit_premask(x, stays_masked);
       }
@@ -144,6 +160,90 @@ std::shared_ptr<Tensor> Linear::fused_forward(const std::shared_ptr<Tensor> &inp
     if (masked) {
       check(mg_free(masked), "free");
     }
+  };
+  return result;
+}
+
+// ---------------------------------------------------------------------------
+// GroupNorm
+// ---------------------------------------------------------------------------
+namespace {
+// A device buffer owned by a closure.
+struct DeviceBuffer {
+  double *ptr = nullptr;
+  explicit DeviceBuffer(size_t n) { check(mg_alloc(n, &ptr), "device allocation"); }
+  ~DeviceBuffer() {
+    if (mg_device() >= 0) {
+      mg_free(ptr);
+    }
+  }
+  DeviceBuffer(const DeviceBuffer &) = delete;
+  DeviceBuffer &operator=(const DeviceBuffer &) = delete;
+};
+}  // namespace
+
+GroupNorm::GroupNorm(size_t groups, size_t channels, double eps) : groups_(groups), channels_(channels), eps_(eps) {
+  if (groups == 0 || channels == 0 || channels % groups != 0) {
+    throw std::invalid_argument("GroupNorm: the channels do not make groups of equal size");
+  }
+  if (!(eps >= 0.0)) {
+    throw std::invalid_argument("GroupNorm: eps must not be negative");
+  }
+  weights_ = std::make_shared<Tensor>(std::vector<size_t>{channels}, std::vector<double>(channels, 1.0));
+  bias_ = std::make_shared<Tensor>(std::vector<size_t>{channels}, std::vector<double>(channels, 0.0));
+}
+
+std::shared_ptr<Tensor> GroupNorm::weights() { return weights_; }
+std::shared_ptr<Tensor> GroupNorm::bias() { return bias_; }
+
+std::shared_ptr<Tensor> GroupNorm::forward(const std::shared_ptr<Tensor> &input, micrograd::Activation activation) {
+  const auto &shape = input->shape();
+  if (shape.size() < 2 || shape.back() != channels_) {
+    throw std::invalid_argument("GroupNorm: input must be [samples, ..., channels]");
+  }
+  size_t positions = 1;
+  for (size_t axis = 1; axis + 1 < shape.size(); axis++) {
+    positions *= shape[axis];
+  }
+  const size_t samples = shape[0], channels = channels_, groups = groups_;
+  const int act = activation == micrograd::Activation::ReLU   ? MG_ACT_RELU
+                  : activation == micrograd::Activation::SiLU ? MG_ACT_SILU
+                                                              : MG_ACT_NONE;
+  auto result = Access::make_result(*input, shape, "group_norm", {input, weights_, bias_});
+  auto stats = std::make_shared<DeviceBuffer>(2 * samples * groups);  // mean, then rstd
+  check(mg_group_norm_fwd(Access::data(*input).device_read(), Access::data(*weights_).device_read(),
+                          Access::data(*bias_).device_read(), Access::data(*result).device_overwrite(), stats->ptr,
+                          stats->ptr + samples * groups, samples, positions, channels, groups, eps_, act),
+        "group norm");
+  Access::backward_fn(*result) = [stats, samples, positions, channels, groups, act](Tensor &self) {
+    if (Access::grad(self).is_zero()) {
+      return;
+    }
+    auto &kids = Access::children(self);
+    Tensor &x = *kids[0];
+    Tensor &w = *kids[1];
+    Tensor &b = *kids[2];
+    const double *g = Access::grad(self).device_read();
+    const double *xv = Access::data(x).device_read();
+    const double *wv = Access::data(w).device_read(), *bv = Access::data(b).device_read();
+    double *gx = nullptr, *gw = nullptr, *gb = nullptr;
+    int flags = 0;
+    bool store = false;
+    if (Access::requires_grad(x)) {
+      gx = Access::grad(x).device_accumulate(&store);
+      flags |= store ? MG_ACC_STORE_A : 0;
+    }
+    if (Access::requires_grad(w)) {
+      gw = Access::grad(w).device_accumulate(&store);
+      flags |= store ? MG_ACC_STORE_B : 0;
+    }
+    if (Access::requires_grad(b)) {
+      gb = Access::grad(b).device_accumulate(&store);
+      flags |= store ? MG_ACC_STORE_C : 0;
+    }
+    check(mg_group_norm_bwd(xv, wv, bv, stats->ptr, stats->ptr + samples * groups, g, gx, gw, gb, samples,
+                            positions, channels, groups, act, flags),
+          "group norm backward");
   };
   return result;
 }
@@ -408,6 +508,80 @@ std::shared_ptr<Tensor> softmax_cross_entropy(const std::shared_ptr<Tensor> &log
   check_logits(logits, labels.size());
   auto ids = std::make_shared<DeviceInts>(labels.data(), labels.size());
   return xent_node(logits, std::move(ids), denom);
+}
+
+// ---------------------------------------------------------------------------
+// Softmax cross-entropy of a linear layer, without its logits
+// ---------------------------------------------------------------------------
+static std::shared_ptr<Tensor> linear_xent_node(const std::shared_ptr<Tensor> &input, Linear &head,
+                                                const std::shared_ptr<DeviceInts> &ids, double denom) {
+  auto w = head.weights(), b = head.bias();
+  const size_t rows = input->shape()[0], in = w->shape()[0], classes = w->shape()[1];
+  if (denom <= 0.0) {
+    denom = static_cast<double>(rows ? rows : 1);
+  }
+  auto result = Access::make_result(*input, {1}, "linear_xent", {input, w, b});
+  const double *xv = Access::data(*input).device_read();
+  const double *wv = Access::data(*w).device_read(), *bv = Access::data(*b).device_read();
+  double *loss = Access::data(*result).device_overwrite();
+  // The gradients for an upstream gradient of 1, in the order of the children.
+  std::vector<std::shared_ptr<DeviceBuffer>> grads(3);
+  if (result->requires_grad()) {
+    const std::shared_ptr<Tensor> kids[3] = {input, w, b};
+    for (int i = 0; i < 3; i++) {
+      if (kids[i]->requires_grad()) {
+        grads[i] = std::make_shared<DeviceBuffer>(kids[i]->size());
+      }
+    }
+    auto at = [&](int i) { return grads[i] ? grads[i]->ptr : nullptr; };
+    check(mg_linear_xent_fwd_bwd(xv, wv, bv, ids->get(), nullptr, loss, at(0), at(1), at(2), rows, in, classes, denom,
+                                 MG_ACC_STORE_A | MG_ACC_STORE_B | MG_ACC_STORE_C),
+          "linear cross-entropy");
+  } else {
+    check(mg_linear_xent_fwd(xv, wv, bv, ids->get(), loss, rows, in, classes, denom), "linear cross-entropy");
+  }
+  Access::data(*result).mirror_async();
+  Access::backward_fn(*result) = [grads](Tensor &self) {
+    if (Access::grad(self).is_zero()) {
+      return;
+    }
+    const double *gl = Access::grad(self).device_read();
+    for (int i = 0; i < 3; i++) {
+      Tensor &kid = *Access::children(self)[i];
+      if (!grads[i] || !Access::requires_grad(kid)) {
+        continue;
+      }
+      bool store = false;
+      double *g = Access::grad(kid).device_accumulate(&store);
+      check(mg_scale_acc(gl, grads[i]->ptr, g, kid.size(), store ? MG_ACC_STORE_A : 0),
+            "linear cross-entropy backward");
+    }
+  };
+  return result;
+}
+
+static void check_head(const std::shared_ptr<Tensor> &input, Linear &head, size_t label_count) {
+  if (input->shape().size() != 2 || input->shape()[1] != head.weights()->shape()[0]) {
+    throw std::invalid_argument("linear_cross_entropy needs 2D inputs of the layer's width");
+  }
+  if (label_count != input->shape()[0]) {
+    throw std::invalid_argument("linear_cross_entropy: one label per row expected");
+  }
+}
+
+std::shared_ptr<Tensor> linear_cross_entropy(const std::shared_ptr<Tensor> &input, Linear &head,
+                                             const std::shared_ptr<Tensor> &labels, double denom) {
+  check_head(input, head, labels->size());
+  auto ids = std::make_shared<DeviceInts>(labels->size());
+  check(mg_f64_to_i32(Access::data(*labels).device_read(), ids->get(), labels->size()), "label conversion");
+  return linear_xent_node(input, head, ids, denom);
+}
+
+std::shared_ptr<Tensor> linear_cross_entropy(const std::shared_ptr<Tensor> &input, Linear &head,
+                                             const std::vector<int> &labels, double denom) {
+  check_head(input, head, labels.size());
+  auto ids = std::make_shared<DeviceInts>(labels.data(), labels.size());
+  return linear_xent_node(input, head, ids, denom);
 }
 
 std::vector<int> argmax_rows(const std::shared_ptr<Tensor> &x) {

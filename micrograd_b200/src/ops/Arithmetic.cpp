@@ -116,6 +116,12 @@ std::shared_ptr<Tensor> Tensor::unary_op(int op, std::string label, double scala
     const bool needs_input = (op == MG_POW || op == MG_RELU);
     const bool needs_output = (op == MG_SIGMOID || op == MG_TANH || op == MG_EXP);
     const double *g = self.grad_.device_read();
+    if (op == MG_RELU && x.data_.packed()) {
+      bool store = false;
+      double *gx = x.grad_.device_accumulate(&store);
+      check(mg_relu_bwd_q8(x.data_.codes(), g, gx, self.size(), store ? MG_ACC_STORE_A : 0), "relu backward");
+      return;
+    }
     const double *a = needs_input ? x.data_.device_read() : nullptr;
     const double *y = needs_output ? self.data_.device_read() : nullptr;
     bool store = false;

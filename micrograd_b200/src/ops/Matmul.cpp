@@ -36,6 +36,11 @@ std::shared_ptr<Tensor> Tensor::matmul(const std::shared_ptr<Tensor> &b) {
       check(mg_gemm_nt(g, bv, ga, m, n, k, store ? 0 : 1, MG_EPI_NONE, nullptr), "matmul dA");
     }
     if (rhs.requires_grad_) {
+      if (lhs.data_.packed()) {
+        double *gb = rhs.grad_.device_accumulate(&store);
+        check(mg_gemm_tn_q8(lhs.data_.codes(), lhs.data_.scales(), g, gb, m, n, k, store ? 0 : 1), "matmul dB");
+        return;
+      }
       const double *av = lhs.data_.device_read();
       double *gb = rhs.grad_.device_accumulate(&store);
       check(mg_gemm_tn(av, g, gb, m, n, k, store ? 0 : 1), "matmul dB");

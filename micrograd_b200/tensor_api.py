@@ -30,6 +30,7 @@ BACKEND_METAL = 1
 
 _BINARY = {"add": 0, "sub": 1, "mul": 2, "div": 3, "matmul": 4}
 _SCALAR = {"add": 0, "sub": 1, "mul": 2, "div": 3, "pow": 4}
+_ACTIVATION = {"none": 0, "relu": 1, "silu": 2}
 _UNARY = {"relu": 0, "sigmoid": 1, "tanh": 2, "sum": 3, "exp": 4}
 
 
@@ -83,6 +84,15 @@ def _declare(lib, extensions: bool) -> None:
             "mgt_comm_world": (C.c_int, []),
             "mgt_argmax_rows": (C.c_int, [vp, _c_int_p, C.c_size_t]),
             "mgt_linear_forward_relu": (vp, [vp, vp]),
+            "mgt_linear_cross_entropy": (vp, [vp, vp, vp, C.c_double]),
+            "mgt_linear_cross_entropy_host": (vp, [vp, vp, _c_int_p, C.c_size_t, C.c_double]),
+            "mgt_norm_new": (vp, [C.c_size_t, C.c_size_t, C.c_double]),
+            "mgt_norm_release": (None, [vp]),
+            "mgt_norm_forward": (vp, [vp, vp, C.c_int]),
+            "mgt_norm_weights": (vp, [vp]),
+            "mgt_norm_bias": (vp, [vp]),
+            "mgt_keep_8bit": (C.c_int, [vp]),
+            "mgt_kept_8bit": (C.c_int, [vp]),
             "mgt_set_requires_grad": (C.c_int, [vp, C.c_int]),
             "mgt_sync": (C.c_int, []),
             "mgt_comm_unique_id": (C.c_int, [C.c_char_p]),
@@ -240,6 +250,12 @@ def bind(path: str) -> SimpleNamespace:
         def set_requires_grad(self, flag: bool) -> None:
             _check(lib.mgt_set_requires_grad(self._h, 1 if flag else 0))
 
+        def keep_8bit(self) -> None:
+            """Tensor::keep_8bit: the values in 8 bits until the backward pass."""
+            _check(lib.mgt_keep_8bit(self._h))
+
+        def kept_8bit(self) -> bool: return bool(lib.mgt_kept_8bit(self._h))
+
         def copy_from_host(self, values) -> None:
             """Tensor::copy_from_host: new values into the device buffer the tensor has."""
             arr = _as_f64(values)
@@ -271,6 +287,25 @@ def bind(path: str) -> SimpleNamespace:
 
         def weights(self) -> Tensor: return Tensor._wrap(lib.mgt_linear_weights(self._h))
         def bias(self) -> Tensor: return Tensor._wrap(lib.mgt_linear_bias(self._h))
+
+    class GroupNorm:
+        """micrograd's GroupNorm: channels last, activation "none", "relu" or "silu"."""
+
+        def __init__(self, groups: int, channels: int, eps: float = 1e-5):
+            self._h = lib.mgt_norm_new(groups, channels, float(eps))
+            if not self._h:
+                _raise()
+
+        def __del__(self):
+            if getattr(self, "_h", None):
+                lib.mgt_norm_release(self._h)
+                self._h = None
+
+        def forward(self, x: Tensor, activation: str = "none") -> Tensor:
+            return Tensor._wrap(lib.mgt_norm_forward(self._h, x._h, _ACTIVATION[activation]))
+
+        def weights(self) -> Tensor: return Tensor._wrap(lib.mgt_norm_weights(self._h))
+        def bias(self) -> Tensor: return Tensor._wrap(lib.mgt_norm_bias(self._h))
 
     class SGD:
         """Mirror of ``class SGD`` (reference include/micrograd/nn.h:23-33)."""
@@ -314,6 +349,15 @@ def bind(path: str) -> SimpleNamespace:
         return Tensor._wrap(lib.mgt_softmax_cross_entropy_host(
             logits._h, ids.ctypes.data_as(_c_int_p), ids.size, float(denom)))
 
+    def linear_cross_entropy(x: Tensor, head: "Linear", labels, denom: float = 0.0) -> Tensor:
+        """Softmax cross-entropy of head.forward(x) without its logits; label -1 leaves a
+        row out.  labels and denom as in softmax_cross_entropy."""
+        if isinstance(labels, Tensor):
+            return Tensor._wrap(lib.mgt_linear_cross_entropy(x._h, head._h, labels._h, float(denom)))
+        ids = np.ascontiguousarray(labels, dtype=np.int32).reshape(-1)
+        return Tensor._wrap(lib.mgt_linear_cross_entropy_host(
+            x._h, head._h, ids.ctypes.data_as(_c_int_p), ids.size, float(denom)))
+
     def from_host(shape, pointer: int) -> Tensor:
         """Tensor::from_host: upload from a raw host address (e.g. pinned memory)."""
         shp = (C.c_size_t * len(shape))(*[int(s) for s in shape])
@@ -354,6 +398,7 @@ def bind(path: str) -> SimpleNamespace:
         lib=lib, extensions=extensions, Tensor=Tensor, Linear=Linear, SGD=SGD,
         mse_loss=mse_loss, avg_pool_2x2=avg_pool_2x2, save_model=save_model,
         load_model=load_model, format_scalar=format_scalar,
+        GroupNorm=GroupNorm if extensions else None, linear_cross_entropy=linear_cross_entropy,
         softmax_cross_entropy=softmax_cross_entropy, argmax_rows=argmax_rows, from_host=from_host,
         comm_rank=lambda: int(lib.mgt_comm_rank()), comm_world=lambda: int(lib.mgt_comm_world()),
         synchronize=synchronize, comm_unique_id=comm_unique_id, comm_init=comm_init,
