@@ -211,7 +211,7 @@ int choose_spans(int tiles, int KT, int sms) {
 // half-width tile (more operand traffic per flop) and for a split contraction
 // (its partial tiles are written and folded: ~22.8 (p+1)/K of the GEMM's time
 // when p partial tiles are written per output tile).
-GemmPlan choose_plan(int M, int N, int K, int sms, int shape, bool divisors_of_112) {
+static GemmPlan choose_plan(int M, int N, int K, int sms, int shape) {
   const int KT = (K + BK - 1) / BK;
   auto tiles_of = [&](int bm, int bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
   if (N <= Skinny16Cfg::BN) {
@@ -258,7 +258,7 @@ GemmPlan choose_plan(int M, int N, int K, int sms, int shape, bool divisors_of_1
   };
   GemmPlan best = cost(half_plan, 1.04) < cost(main_plan, 1.0) ? half_plan : main_plan;
   double best_cost = best.tile == kTileHalf ? cost(half_plan, 1.04) : cost(main_plan, 1.0);
-  if (divisors_of_112 && M % MainCfg::BM != 0 && M % Rows112Cfg::BM == 0) {
+  if (M % MainCfg::BM != 0 && M % Rows112Cfg::BM == 0) {
     GemmPlan p112{kTileRows112, Rows112Cfg::BM, Rows112Cfg::BN,
                   choose_spans(tiles_of(Rows112Cfg::BM, Rows112Cfg::BN), KT, sms)};
     if (cost(p112, 1.02) < best_cost) {
@@ -266,7 +266,7 @@ GemmPlan choose_plan(int M, int N, int K, int sms, int shape, bool divisors_of_1
       best_cost = cost(p112, 1.02);
     }
   }
-  if (divisors_of_112 && N % MainCfg::BN != 0 && N % Cols112Cfg::BN == 0) {
+  if (N % MainCfg::BN != 0 && N % Cols112Cfg::BN == 0) {
     GemmPlan c112{kTileCols112, Cols112Cfg::BM, Cols112Cfg::BN,
                   choose_spans(tiles_of(Cols112Cfg::BM, Cols112Cfg::BN), KT, sms)};
     if (cost(c112, 1.02) < best_cost) best = c112;

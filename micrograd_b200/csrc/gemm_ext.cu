@@ -25,35 +25,76 @@ template <bool AK, bool BK_> static int launch_layout_ext(int tile, const DmmaLa
   }
 }
 
-// Few rows go to tiles of few rows, unless the columns are few as well.
+constexpr int kFoldBySegments = 6;  // split tiles are folded by a kernel of its own from here on
+
+// Tile and split of a problem, by choose_plan's cost (rounds of CTAs x work per CTA plus
+// 3.3 us per CTA), with the small tiles among the candidates: problems that leave SMs idle
+// on large ones, and those of few rows.  A small tile moves more bytes per flop, from L2
+// where the problem is small; the handicaps are the ratio of its copy time at 148 SMs to
+// its tensor time.
 static GemmPlan plan_ext(int M, int N, int K, int sms) {
-  if (M <= 64 && N > SkinnyCfg::BN) {
-    GemmPlan p = M <= 16 ? GemmPlan{kTileRows16, 16, 128, 0}
-                         : (M <= 32 ? GemmPlan{kTileRows32, 32, 128, 0} : GemmPlan{kTileRows64, 64, 128, 0});
-    p.spans = choose_spans((N + 127) / 128, (K + BK - 1) / BK, sms);
-    return p;
+  struct Candidate {
+    int tile, bm, bn;
+    double handicap;
+  };
+  static const Candidate candidates[] = {
+      {kTileMain, 128, 128, 1.0},   {kTileHalf, 128, 64, 1.04},    {kTileRows64, 64, 128, 1.06},
+      {kTileRows32, 32, 128, 1.3},  {kTileSkinny, 128, 32, 1.3},   {kTileRows16, 16, 128, 1.7},
+      {kTileSkinny16, 128, 16, 1.7},
+  };
+  const int KT = (K + BK - 1) / BK;
+  GemmPlan best{};
+  double best_cost = 0.0;
+  for (const Candidate &c : candidates) {
+    const long long tiles = (long long)((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn);
+    if (tiles >= (1ll << 30)) continue;
+    const GemmPlan p{c.tile, c.bm, c.bn, choose_spans((int)tiles, KT, sms)};
+    const double kt = (double)c.bm * c.bn * c.handicap, per_cta = 25800.0;
+    double cost;
+    if (p.spans == 0) {
+      cost = (double)((tiles + sms - 1) / sms) * (kt * KT + per_cta);
+    } else {
+      const double work = (double)tiles * KT / p.spans, segments = (double)tiles / p.spans + 1.0;
+      cost = (work * kt + segments * per_cta) * (tiles >= sms ? 1.04 : 1.0);
+      // the fold: by all SMs in a launch of its own, or one CTA per tile
+      cost += p.spans >= kFoldBySegments * tiles ? 25800.0 : 4000.0 * p.spans / (double)tiles * c.bm * c.bn / 16384.0;
+    }
+    if (best_cost == 0.0 || cost < best_cost) {
+      best = p;
+      best_cost = cost;
+    }
   }
-  return choose_plan(M, N, K, sms, 2, false);
+  return best;
 }
 
-// Adds up the partial tiles of split tiles, in slot (= k) order, a thread per output
-// element, and runs the epilogue.  The kernel's own fold has one CTA per tile, which is
+// Adds up the partial tiles of split tiles in a fixed order (that of k within an eighth of
+// the segments, then the eighths) and runs the epilogue.  The kernel's own fold has one CTA per tile, which is
 // right for many tiles; for few it is the longest part: 148 partial tiles of 128 x 64
 // take one CTA over 100 us and all SMs 4.
-constexpr int kFoldBySegments = 6;  // fold here from this many segments per tile on
-
 __global__ void __launch_bounds__(256)
 fold_tiles_kernel(GemmEpilogue ep, const int2 *__restrict__ tiles, int tiles_n, int bm, int bn, int M, int N) {
+  __shared__ double part[8][33];
   const int2 info = tiles[blockIdx.y];
   if (info.y == 0) return;  // a whole tile: written by the kernel itself
-  const int e = blockIdx.x * 256 + threadIdx.x, r = e / bn, c = e - r * bn;
+  // 32 elements per CTA; its eight warps take consecutive eighths of the segments.
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int e = blockIdx.x * 32 + lane, r = e / bn, c = e - r * bn;
   const int row = (blockIdx.y / tiles_n) * bm + r, col = (blockIdx.y % tiles_n) * bn + c;
-  if (r >= bm || row >= M || col >= N) return;
+  const bool in = row < M && col < N;
   const size_t slot = (size_t)bm * bn;
-  const double *part = ep.partial + info.x * slot + e;
+  const double *src = ep.partial + info.x * slot + e;
+  const int first = info.y * warp / 8, last = info.y * (warp + 1) / 8;
   double v = 0.0;
+  if (in) {
 #pragma unroll 8
-  for (int k = 0; k < info.y; k++) v += __ldcs(part + k * slot);
+    for (int k = first; k < last; k++) v += __ldcs(src + k * slot);
+  }
+  part[warp][lane] = v;
+  __syncthreads();
+  if (warp != 0 || !in) return;
+  v = 0.0;
+#pragma unroll
+  for (int w = 0; w < 8; w++) v += part[w][lane];
   if (ep.mode == MG_EPI_BIAS || ep.mode == MG_EPI_BIAS_RELU) v += __ldg(ep.aux + col);
   if (ep.mode == MG_EPI_BIAS_RELU) v = v > 0 ? v : 0.0;
   if (ep.mask8) v = v * (ep.mask8[(size_t)row * ep.ld_mask8 + col] > 0 ? 1.0 : 0.0);
@@ -122,7 +163,7 @@ int run_gemm_ext(const GemmExt &e) {
   const GemmPlan plan = plan_ext(M, N, K, c.sm_count);
   const int tiles_m = (M + plan.bm - 1) / plan.bm, tiles_n = (N + plan.bn - 1) / plan.bn;
   const bool fold_here = plan.spans >= kFoldBySegments * tiles_m * tiles_n;
-  if (!e.mask8 && dense && !fold_here && (d.M > 64 || d.N <= (size_t)SkinnyCfg::BN)) return run_gemm(d);
+  if (!e.mask8 && dense && !fold_here && (plan.tile == kTileMain || plan.tile == kTileHalf)) return run_gemm(d);
   if ((lda & 1) || off_16_bytes(d.A) || (ldb & 1) || off_16_bytes(d.B))
     return fail(MG_ERR_INVALID, "gemm: operand rows do not start on 16-byte boundaries");
   DmmaLaunch L{};
@@ -180,7 +221,7 @@ int run_gemm_ext(const GemmExt &e) {
   else if (d.a_kcontig) rc = launch_layout_ext<true, true>(plan.tile, L);
   else rc = launch_layout_ext<false, false>(plan.tile, L);
   if (rc != MG_OK || !split || !fold_here) return rc;
-  fold_tiles_kernel<<<dim3((unsigned)((plan.bm * plan.bn + 255) / 256), (unsigned)(tiles_m * tiles_n)), 256, 0,
+  fold_tiles_kernel<<<dim3((unsigned)(plan.bm * plan.bn / 32), (unsigned)(tiles_m * tiles_n)), 256, 0,
                       c.stream>>>(ep, table->dev_tiles, tiles_n, plan.bm, plan.bn, M, N);
   MG_LAUNCH_CHECK("gemm fold");
   return MG_OK;

@@ -734,7 +734,6 @@ struct SegTable {
 };
 
 int choose_spans(int tiles, int KT, int sms);
-GemmPlan choose_plan(int M, int N, int K, int sms, int shape, bool divisors_of_112 = true);
 int seg_table_for(int tiles_m, int tiles_n, int KT, int bm, int bn, int spans, const SegTable **out);
 
 }  // namespace mg

@@ -288,7 +288,361 @@ struct Head {
   bool grad;
 };
 
+// ---------------------------------------------------------------------------
+// Up to four rows (a single one in the per-sample loop): everything is a stream over w, so no
+// tile of the tensor kernel is worth filling.  A CTA takes a slab of 64 classes.
+//   1. z = x w + bias of the slab, each warp every eighth row of w, and the slab's
+//      (max, sum of exp) per row; the CTA that finishes last joins the slabs (in order)
+//      to each row's (max, sum) and the loss.
+//   2. p of the slab; gw and gbias of its classes, and its share of gx.
+//   3. gx: the slabs' shares, in order.
+// Left-out rows count as zeros of x and p, whatever x holds.
+// ---------------------------------------------------------------------------
+constexpr int kFewRows = 4, kSlab = 64, kFewThreads = 256, kFewWarps = kFewThreads / 32, kFewK = 128;
+
+struct FewRows {
+  const double *x, *w, *bias;
+  const int *labels;
+  const double *gloss;
+  double *loss, *gx, *gw, *gbias;
+  double *z, *slabs, *at_label, *rows, *shares;  // workspace: [M][Vp], [slabs][M][2], [M], [M][2], [slabs][M][K]
+  int M, K, V;
+  size_t Vp;
+  double inv_denom;
+  bool acc_x, acc_w, acc_b, grad;
+  unsigned int *ticket;
+  int *status;
+};
+
+__device__ __forceinline__ bool few_keep(const FewRows &a, int i) {
+  return i < a.M && a.labels[i] >= 0 && a.labels[i] < a.V;
+}
+
+// w's values of the lane's two classes in the row at src.  Lanes without classes read the
+// last ones (a conditional load would be waited for where it meets its default).
+template <bool PAIR> __device__ __forceinline__ void few_load(const double *src, int c0, int c1, int V, double &w0, double &w1) {
+  if (PAIR) {
+    const double2 t = __ldg(reinterpret_cast<const double2 *>(src + (c0 < V ? c0 : V - 2)));
+    w0 = t.x;
+    w1 = t.y;
+  } else {
+    w0 = __ldg(src + (c0 < V ? c0 : V - 1));
+    w1 = __ldg(src + (c1 < V ? c1 : V - 1));
+  }
+}
+
+// The lane's two classes of a slab: neighbours where w's rows allow pairs, 32 apart else.
+template <bool PAIR> __device__ __forceinline__ int few_class(int lane, int j) {
+  return PAIR ? 2 * lane + j : lane + 32 * j;
+}
+
+template <int MR, bool PAIR>
+__global__ void __launch_bounds__(kFewThreads) few_rows_fwd_kernel(const FewRows a) {
+  __shared__ double xs[kFewK][MR];
+  __shared__ double sums[kFewWarps][MR][kSlab];
+  __shared__ double red[32];
+  __shared__ bool is_last;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, v0 = blockIdx.x * kSlab;
+  const int c0 = v0 + few_class<PAIR>(lane, 0), c1 = v0 + few_class<PAIR>(lane, 1);
+  double acc[MR][2];
+#pragma unroll
+  for (int i = 0; i < MR; i++) acc[i][0] = acc[i][1] = 0.0;
+  constexpr int kRowsPerWarp = kFewK / kFewWarps;
+  for (int k0 = 0; k0 < a.K; k0 += kFewK) {
+    const int ks = a.K - k0 < kFewK ? a.K - k0 : kFewK;
+    // All of the warp's rows of w are on their way before x is waited for.
+    double w0[kRowsPerWarp], w1[kRowsPerWarp];
+#pragma unroll
+    for (int r = 0; r < kRowsPerWarp; r++) {
+      const int k = warp + r * kFewWarps < ks ? warp + r * kFewWarps : ks - 1;
+      few_load<PAIR>(a.w + (size_t)(k0 + k) * a.V, c0, c1, a.V, w0[r], w1[r]);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < kFewK * MR; e += kFewThreads) {
+      const int i = e / kFewK, k = e % kFewK;
+      xs[k][i] = i < a.M && k < ks ? a.x[(size_t)i * a.K + k0 + k] : 0.0;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kRowsPerWarp; r++) {
+      if (warp + r * kFewWarps < ks) {
+#pragma unroll
+        for (int i = 0; i < MR; i++) {
+          const double x = xs[warp + r * kFewWarps][i];
+          acc[i][0] = fma(x, w0[r], acc[i][0]);
+          acc[i][1] = fma(x, w1[r], acc[i][1]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < MR; i++) {
+    sums[warp][i][few_class<PAIR>(lane, 0)] = acc[i][0];
+    sums[warp][i][few_class<PAIR>(lane, 1)] = acc[i][1];
+  }
+  __syncthreads();
+  // A warp per row: its 64 logits, two per lane.
+  for (int i = warp; i < a.M; i += kFewWarps) {
+    double z[2];
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      const int s = lane + 32 * j, c = v0 + s;
+      z[j] = -INFINITY;
+      if (c < a.V) {
+        double t = 0.0;
+#pragma unroll
+        for (int w = 0; w < kFewWarps; w++) t += sums[w][i][s];
+        if (a.bias) t += a.bias[c];
+        z[j] = t;
+        if (a.grad) a.z[(size_t)i * a.Vp + c] = t;
+        if (c == a.labels[i]) a.at_label[i] = t;
+      }
+    }
+    double top = fmax(z[0], z[1]);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, off));
+    // (a slab of classes without probability adds nothing; a NaN is in the sum)
+    double sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < 2; j++) sum += z[j] == -INFINITY ? 0.0 : exp(z[j] - top);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    if (lane == 0) {
+      double *out = a.slabs + ((size_t)blockIdx.x * a.M + i) * 2;
+      out[0] = top;
+      out[1] = sum;
+    }
+  }
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) is_last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
+  __syncthreads();
+  if (!is_last) return;
+  __threadfence();
+  for (int i = warp; i < a.M; i += kFewWarps) {
+    const bool keep = few_keep(a, i);
+    double top = -INFINITY;
+    for (unsigned s = lane; s < gridDim.x; s += 32) top = fmax(top, __ldcg(a.slabs + ((size_t)s * a.M + i) * 2));
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, off));
+    double sum = 0.0;
+    for (unsigned s = lane; s < gridDim.x; s += 32) {
+      const double *p = a.slabs + ((size_t)s * a.M + i) * 2;
+      sum += __ldcg(p + 1) * exp(__ldcg(p) - top);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    if (lane == 0) {
+      a.rows[2 * i] = top;
+      a.rows[2 * i + 1] = sum;
+      red[i] = keep ? -(__ldcg(a.at_label + i) - top - log(sum)) : 0.0;
+      if (!keep && a.labels[i] != -1) atomicExch(a.status, 101);  // not a class and not "left out"
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double loss = 0.0;
+    for (int i = 0; i < a.M; i++) loss += red[i];
+    a.loss[0] = loss * a.inv_denom;
+    *a.ticket = 0u;
+  }
+}
+
+template <int MR, bool PAIR>
+__global__ void __launch_bounds__(kFewThreads) few_rows_bwd_kernel(const FewRows a) {
+  constexpr int kPitch = kSlab + 4;  // eight rows x four classes 4 apart fall into different banks
+  __shared__ double xs[kSlab][MR];
+  __shared__ __align__(16) double ps[kSlab][MR];
+  __shared__ double ws[kSlab][kPitch];
+  __shared__ bool kept[MR];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, v0 = blockIdx.x * kSlab;
+  const int s0 = few_class<PAIR>(lane, 0), s1 = few_class<PAIR>(lane, 1), c0 = v0 + s0, c1 = v0 + s1;
+  constexpr int kRowsPerWarp = kSlab / kFewWarps;
+  // Rows k0 ... of w (64 at a time), asked for one step ahead.
+  double w0[kRowsPerWarp], w1[kRowsPerWarp];
+  auto fetch = [&](int k0) {
+#pragma unroll
+    for (int r = 0; r < kRowsPerWarp; r++) {
+      const int k = k0 + warp + r * kFewWarps < a.K ? k0 + warp + r * kFewWarps : a.K - 1;
+      few_load<PAIR>(a.w + (size_t)k * a.V, c0, c1, a.V, w0[r], w1[r]);
+    }
+  };
+  constexpr int kXs = (kSlab * MR + kFewThreads - 1) / kFewThreads;
+  double x_next[kXs];
+  auto fetch_x = [&](int k0) {
+#pragma unroll
+    for (int r = 0; r < kXs; r++) {
+      const int e = threadIdx.x + r * kFewThreads, i = e / kSlab < a.M ? e / kSlab : 0, k = k0 + (e & (kSlab - 1));
+      x_next[r] = __ldg(a.x + (size_t)i * a.K + (k < a.K ? k : a.K - 1));
+    }
+  };
+  if (threadIdx.x < MR) kept[threadIdx.x] = few_keep(a, threadIdx.x);
+  if (a.gx) fetch(0);
+  if (a.K) fetch_x(0);
+  __syncthreads();
+  const double c = (a.gloss ? *a.gloss : 1.0) * a.inv_denom;
+  for (int e = threadIdx.x; e < kSlab * MR; e += kFewThreads) {
+    const int i = e / kSlab, s = e - i * kSlab, v = v0 + s;
+    double p = 0.0;
+    if (v < a.V && kept[i]) {
+      const double scale = c / a.rows[2 * i + 1];
+      p = exp(a.z[(size_t)i * a.Vp + v] - a.rows[2 * i]);
+      p = v == a.labels[i] ? fma(p, scale, -c) : p * scale;
+    }
+    ps[s][i] = p;
+  }
+  __syncthreads();
+  if (a.gbias && threadIdx.x < kSlab && v0 + (int)threadIdx.x < a.V) {
+    double s = 0.0;
+    for (int i = 0; i < a.M; i++) s += ps[threadIdx.x][i];
+    double *dst = a.gbias + v0 + threadIdx.x;
+    *dst = a.acc_b ? *dst + s : s;
+  }
+  double p0[MR], p1[MR];
+#pragma unroll
+  for (int i = 0; i < MR; i++) {
+    p0[i] = ps[s0][i];
+    p1[i] = ps[s1][i];
+  }
+  for (int k0 = 0; k0 < a.K; k0 += kSlab) {
+    const int ks = a.K - k0 < kSlab ? a.K - k0 : kSlab;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kXs; r++) {
+      const int e = threadIdx.x + r * kFewThreads, i = e / kSlab, k = e & (kSlab - 1);
+      if (i < MR) xs[k][i] = k < ks && kept[i] ? x_next[r] : 0.0;
+    }
+    if (k0 + kSlab < a.K) fetch_x(k0 + kSlab);
+    if (a.gx) {
+#pragma unroll
+      for (int r = 0; r < kRowsPerWarp; r++) {
+        // (classes behind the last one have p = 0, but w there may be anything)
+        ws[warp + r * kFewWarps][s0] = c0 < a.V ? w0[r] : 0.0;
+        ws[warp + r * kFewWarps][s1] = c1 < a.V ? w1[r] : 0.0;
+      }
+      if (k0 + kSlab < a.K) fetch(k0 + kSlab);
+    }
+    __syncthreads();
+    if (a.gw) {
+#pragma unroll 4
+      for (int k = warp; k < ks; k += kFewWarps) {
+        double g0 = 0.0, g1 = 0.0;
+#pragma unroll
+        for (int i = 0; i < MR; i++) {
+          g0 = fma(xs[k][i], p0[i], g0);
+          g1 = fma(xs[k][i], p1[i], g1);
+        }
+        double *dst = a.gw + (size_t)(k0 + k) * a.V;
+        if (PAIR) {
+          if (c0 < a.V) {
+            double2 *d = reinterpret_cast<double2 *>(dst + c0);
+            if (a.acc_w) {
+              const double2 o = *d;
+              g0 = o.x + g0;
+              g1 = o.y + g1;
+            }
+            __stcs(d, make_double2(g0, g1));
+          }
+        } else {
+          if (c0 < a.V) dst[c0] = a.acc_w ? dst[c0] + g0 : g0;
+          if (c1 < a.V) dst[c1] = a.acc_w ? dst[c1] + g1 : g1;
+        }
+      }
+    }
+    if (a.gx) {
+      // Four lanes share a row of w, every fourth class each.
+      const int k = warp * 8 + (lane >> 2), q = lane & 3;
+      double s[MR];
+#pragma unroll
+      for (int i = 0; i < MR; i++) s[i] = 0.0;
+#pragma unroll
+      for (int v = 0; v < kSlab; v += 4) {
+        const double w = ws[k][v + q];
+#pragma unroll
+        for (int i = 0; i < MR; i++) s[i] = fma(w, ps[v + q][i], s[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < MR; i++) {
+        s[i] += __shfl_xor_sync(0xffffffffu, s[i], 1);
+        s[i] += __shfl_xor_sync(0xffffffffu, s[i], 2);
+        if ((i & 3) == q && i < a.M && k < ks)
+          a.shares[((size_t)blockIdx.x * a.M + i) * a.K + k0 + k] = s[i];
+      }
+    }
+  }
+}
+
+// gx[i] (+)= sum over the slabs of shares[slab][i]: 16 entries per CTA, 16 threads each.
+__global__ void __launch_bounds__(256)
+few_rows_gx_kernel(const double *__restrict__ shares, unsigned slabs, size_t n, double *gx, bool accumulate) {
+  __shared__ double part[16][17];
+  const int e = threadIdx.x & 15, t = threadIdx.x >> 4;
+  const size_t at = (size_t)blockIdx.x * 16 + e;
+  double s = 0.0;
+  if (at < n) {
+#pragma unroll 8
+    for (unsigned k = t; k < slabs; k += 16) s += __ldcs(shares + k * n + at);
+  }
+  part[t][e] = s;
+  __syncthreads();
+  if (t == 0 && at < n) {
+    s = 0.0;
+    for (int k = 0; k < 16; k++) s += part[k][e];
+    gx[at] = accumulate ? gx[at] + s : s;
+  }
+}
+
+template <int MR> static int launch_few(const FewRows &a, bool pair) {
+  Context &c = ctx();
+  const unsigned slabs = (unsigned)((a.V + kSlab - 1) / kSlab);
+  if (pair) few_rows_fwd_kernel<MR, true><<<slabs, kFewThreads, 0, c.stream>>>(a);
+  else few_rows_fwd_kernel<MR, false><<<slabs, kFewThreads, 0, c.stream>>>(a);
+  MG_LAUNCH_CHECK("linear_xent (few rows)");
+  if (!a.grad) return MG_OK;
+  if (pair) few_rows_bwd_kernel<MR, true><<<slabs, kFewThreads, 0, c.stream>>>(a);
+  else few_rows_bwd_kernel<MR, false><<<slabs, kFewThreads, 0, c.stream>>>(a);
+  MG_LAUNCH_CHECK("linear_xent (few rows, gradients)");
+  if (!a.gx) return MG_OK;
+  const size_t n = (size_t)a.M * a.K;
+  few_rows_gx_kernel<<<(unsigned)((n + 15) / 16), 256, 0, c.stream>>>(a.shares, slabs, n, a.gx, a.acc_x);
+  MG_LAUNCH_CHECK("linear_xent (few rows, gx)");
+  return MG_OK;
+}
+
+static int run_few_rows(const Head &h) {
+  Context &c = ctx();
+  FewRows a{};
+  a.x = h.x; a.w = h.w; a.bias = h.bias; a.labels = h.labels; a.gloss = h.gloss; a.loss = h.loss;
+  a.gx = h.K ? h.gx : nullptr; a.gw = h.K ? h.gw : nullptr; a.gbias = h.gbias;
+  a.M = (int)h.M; a.K = (int)h.K; a.V = (int)h.V;
+  a.Vp = pitch16(h.V);
+  a.inv_denom = 1.0 / h.denom;
+  a.acc_x = !(h.flags & MG_ACC_STORE_A);
+  a.acc_w = !(h.flags & MG_ACC_STORE_B);
+  a.acc_b = !(h.flags & MG_ACC_STORE_C);
+  a.grad = h.grad;
+  a.ticket = c.reduce_ticket + 1;
+  a.status = c.kernel_status;
+  const size_t slabs = (h.V + kSlab - 1) / kSlab;
+  double *ws = nullptr;
+  const size_t n_z = h.grad ? h.M * a.Vp : 0, n_slabs = slabs * h.M * 2, n_rows = 3 * h.M;
+  int rc = mg_alloc(n_z + n_slabs + n_rows + (a.gx ? slabs * h.M * h.K : 0), &ws);
+  if (rc != MG_OK) return rc;
+  a.z = ws;
+  a.slabs = ws + n_z;
+  a.at_label = a.slabs + n_slabs;
+  a.rows = a.at_label + h.M;
+  a.shares = a.rows + 2 * h.M;
+  const bool pair = h.V % 2 == 0 && !off_16_bytes(h.w) && !(a.gw && off_16_bytes(a.gw));
+  if (h.M == 1) rc = launch_few<1>(a, pair);
+  else if (h.M == 2) rc = launch_few<2>(a, pair);
+  else rc = launch_few<4>(a, pair);
+  const int freed = mg_free(ws);
+  return rc != MG_OK ? rc : freed;
+}
+
 static int run_head(const Head &h) {
+  if (h.M <= (size_t)kFewRows) return run_few_rows(h);
   Context &c = ctx();
   // The tensor kernel takes operand rows of an even number of doubles from 16-byte
   // boundaries.  x and w that do not come like that are copied into rows that do (M K
