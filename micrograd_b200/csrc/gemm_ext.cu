@@ -21,6 +21,7 @@ template <bool AK, bool BK_> static int launch_layout_ext(int tile, const DmmaLa
     case kTileRows16: return launch_ext<AK, BK_, Rows16Cfg>(L);
     case kTileRows32: return launch_ext<AK, BK_, Rows32Cfg>(L);
     case kTileRows64: return launch_ext<AK, BK_, Rows64Cfg>(L);
+    case kTileRows112: return launch_ext<AK, BK_, Rows112Cfg>(L);
     default: return launch_ext<AK, BK_, MainCfg>(L);
   }
 }
@@ -38,7 +39,7 @@ static GemmPlan plan_ext(int M, int N, int K, int sms) {
     double handicap;
   };
   static const Candidate candidates[] = {
-      {kTileMain, 128, 128, 1.0},   {kTileHalf, 128, 64, 1.04},    {kTileRows64, 64, 128, 1.06},
+      {kTileMain, 128, 128, 1.0},   {kTileHalf, 128, 64, 1.04},    {kTileRows112, 112, 128, 1.06}, {kTileRows64, 64, 128, 1.06},
       {kTileRows32, 32, 128, 1.3},  {kTileSkinny, 128, 32, 1.3},   {kTileRows16, 16, 128, 1.7},
       {kTileSkinny16, 128, 16, 1.7},
   };
@@ -163,7 +164,11 @@ int run_gemm_ext(const GemmExt &e) {
   const GemmPlan plan = plan_ext(M, N, K, c.sm_count);
   const int tiles_m = (M + plan.bm - 1) / plan.bm, tiles_n = (N + plan.bn - 1) / plan.bn;
   const bool fold_here = plan.spans >= kFoldBySegments * tiles_m * tiles_n;
-  if (!e.mask8 && dense && !fold_here && (plan.tile == kTileMain || plan.tile == kTileHalf)) return run_gemm(d);
+  // Where a large tile is right and the matrices are dense, gemm.cu's instantiations and
+  // its own choice among the large tiles are the faster ones.
+  if (!e.mask8 && dense && !fold_here &&
+      (plan.tile == kTileMain || plan.tile == kTileHalf || plan.tile == kTileRows112))
+    return run_gemm(d);
   if ((lda & 1) || off_16_bytes(d.A) || (ldb & 1) || off_16_bytes(d.B))
     return fail(MG_ERR_INVALID, "gemm: operand rows do not start on 16-byte boundaries");
   DmmaLaunch L{};

@@ -15,231 +15,143 @@
 #include "common.cuh"
 #include "gemm.cuh"
 
-#include <cooperative_groups.h>
-
 namespace mg {
 
 // Logits held at a time.
 constexpr size_t kBlockBytes = (size_t)1 << 30;
 
-__device__ __forceinline__ double block_reduce(double v, bool take_max, double *smem32) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+__device__ __forceinline__ double warp_max(double v) {
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    const double o = __shfl_xor_sync(0xffffffffu, v, off);
-    v = take_max ? fmax(v, o) : v + o;
-  }
-  __syncthreads();
-  if (lane == 0) smem32[warp] = v;
-  __syncthreads();
-  const int warps = blockDim.x >> 5;
-  v = lane < warps ? smem32[lane] : (take_max ? -INFINITY : 0.0);
+  for (int off = 16; off > 0; off >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, off));
+  return v;
+}
+__device__ __forceinline__ double warp_total(double v) {
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    const double o = __shfl_xor_sync(0xffffffffu, v, off);
-    v = take_max ? fmax(v, o) : v + o;
-  }
+  for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
   return v;
 }
 
-// Over the CS CTAs of a row; slot is double-buffered by the two calls a row makes.
-template <int CS> __device__ __forceinline__ double row_reduce(double v, bool take_max, double *smem32, double *slot) {
-  v = block_reduce(v, take_max, smem32);
-  if (CS == 1) return v;
-  auto cluster = cooperative_groups::this_cluster();
-  if (threadIdx.x == 0) *slot = v;
-  cluster.sync();
-  double all = take_max ? -INFINITY : 0.0;
+// The block's softmax in three passes without a barrier in any of them: a warp per 512
+// classes of a row leaves their (max, sum of exp); a warp per row joins those; then a
+// thread per pair of classes walks down the rows, which turns the logits into p and adds
+// up the bias gradient on the way.  24 bytes of traffic and two exponentials per logit:
+// 777 x 50 257 takes 236 us with the bias gradient.  Rows held in the registers of a
+// cluster of CTAs (16 bytes, one exponential, and a pass of its own for the bias
+// gradient) took 304: two CTAs fit an SM, and each waits for its loads, two cluster
+// barriers and its stores in turn.
+constexpr int kSegment = 512;  // classes per warp: 16 per lane
+
+__global__ void __launch_bounds__(256)
+xent_segments_kernel(const double *__restrict__ z, size_t pitch, size_t rows, int V, unsigned segments,
+                     double2 *__restrict__ out) {
+  const int lane = threadIdx.x & 31;
+  const size_t all = rows * segments;
+  for (size_t at = ((size_t)blockIdx.x * 256 + threadIdx.x) >> 5; at < all; at += (size_t)gridDim.x * 8) {
+    const size_t row = at / segments;
+    const int j0 = (int)(at - row * segments) * kSegment + lane * 4;
+    const double *r = z + row * pitch;
+    double v[16];
 #pragma unroll
-  for (int r = 0; r < CS; r++) {
-    const double o = *cluster.map_shared_rank(slot, r);
-    all = take_max ? fmax(all, o) : all + o;
+    for (int i = 0; i < 4; i++) {
+      // (lanes behind the end read the row's first classes: the pitch is a multiple of 16)
+      const int j = j0 + 128 * i;
+      const double4v q = *reinterpret_cast<const double4v *>(r + (j < V ? j : 0));
+      v[4 * i] = j < V ? q.x : -INFINITY;
+      v[4 * i + 1] = j + 1 < V ? q.y : -INFINITY;
+      v[4 * i + 2] = j + 2 < V ? q.z : -INFINITY;
+      v[4 * i + 3] = j + 3 < V ? q.w : -INFINITY;
+    }
+    double top = v[0];
+#pragma unroll
+    for (int i = 1; i < 16; i++) top = fmax(top, v[i]);
+    top = warp_max(top);
+    // (classes without probability add nothing, also where a segment has no others; a
+    // NaN is in the sum)
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < 16; i++) sum += v[i] == -INFINITY ? 0.0 : exp(v[i] - top);
+    sum = warp_total(sum);
+    if (lane == 0) out[at] = make_double2(top, sum);
   }
-  return all;
 }
 
-// A row's loss and, when GRAD, its logits replaced by p.  CS CTAs (a cluster) share a
-// row: each keeps its part, a contiguous piece of `piece` classes (a multiple of 4, at
-// most kRowsThreads x kRowsValues), in registers, so that a logit is read once, its
-// exponential computed once and p written once.  What is between V and the pitch is
-// neither used nor written.
-constexpr int kRowsThreads = 512, kRowsValues = 16;
-
-template <bool GRAD, int CS>
-__global__ void __launch_bounds__(kRowsThreads, 2)
-xent_rows_kernel(double *__restrict__ z, const int *__restrict__ labels, const double *__restrict__ gloss,
-                 double *__restrict__ row_loss, int V, size_t pitch, int piece, double inv_denom, int *status) {
-  __shared__ double smem32[32];
-  __shared__ double slot[2];
-  const size_t row = blockIdx.x / CS;
-  const int rank = CS > 1 ? (int)(blockIdx.x % CS) : 0;
-  const int begin = rank * piece, end = begin + piece < V ? begin + piece : V;
-  double *r = z + row * pitch;
+// row_stats[i] = (max, gloss / denom / sum), or (0, 0) for a row that is left out;
+// row_loss[i].
+__global__ void __launch_bounds__(256)
+xent_join_kernel(const double *__restrict__ z, size_t pitch, const double2 *__restrict__ parts, unsigned segments,
+                 const int *__restrict__ labels, const double *__restrict__ gloss, size_t rows, int V,
+                 double inv_denom, double2 *__restrict__ row_stats, double *__restrict__ row_loss, int *status) {
+  const int lane = threadIdx.x & 31;
+  const size_t row = ((size_t)blockIdx.x * 256 + threadIdx.x) >> 5;
+  if (row >= rows) return;
   const int label = labels[row];
   const bool keep = label >= 0 && label < V;
-  if (!keep) {  // (the same in all CTAs of the row)
-    if (threadIdx.x == 0 && rank == 0) {
-      if (label != -1) atomicExch(status, 101);  // not a class and not "left out"
-      row_loss[row] = 0.0;
-    }
-    if (GRAD)
-      for (int j = begin + threadIdx.x; j < end; j += kRowsThreads) r[j] = 0.0;
-    return;
-  }
-  double v[kRowsValues];
   double top = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < kRowsValues / 4; i++) {
-    const int j = begin + (i * kRowsThreads + threadIdx.x) * 4;
-    double4v q{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-    if (j < end) q = *reinterpret_cast<const double4v *>(r + j);  // (the pitch is a multiple of 16)
-    v[4 * i] = q.x;
-    v[4 * i + 1] = j + 1 < end ? q.y : -INFINITY;
-    v[4 * i + 2] = j + 2 < end ? q.z : -INFINITY;
-    v[4 * i + 3] = j + 3 < end ? q.w : -INFINITY;
-  }
-#pragma unroll
-  for (int i = 0; i < kRowsValues; i++) top = fmax(top, v[i]);
-  top = row_reduce<CS>(top, true, smem32, &slot[0]);
-  const double at_label = threadIdx.x == 0 && rank == 0 ? r[label] : 0.0;
+  for (unsigned s = lane; s < segments; s += 32) top = fmax(top, parts[row * segments + s].x);
+  top = warp_max(top);
   double sum = 0.0;
-#pragma unroll
-  for (int i = 0; i < kRowsValues; i++) {
-    const int j = begin + ((i >> 2) * kRowsThreads + threadIdx.x) * 4 + (i & 3);
-    if (j < end) {
-      v[i] = exp(v[i] - top);
-      sum += v[i];
-    }
+  for (unsigned s = lane; s < segments; s += 32) {
+    const double2 p = parts[row * segments + s];
+    sum += p.y * exp(p.x - top);
   }
-  // (p is written only after every CTA of the row has passed this meeting point, so
-  // the label's logit has been read)
-  sum = row_reduce<CS>(sum, false, smem32, &slot[1]);
-  if (threadIdx.x == 0 && rank == 0) row_loss[row] = -(at_label - top - log(sum));
-  if (GRAD) {
-    const double c = (gloss ? *gloss : 1.0) * inv_denom, scale = c / sum;
-#pragma unroll
-    for (int i = 0; i < kRowsValues / 4; i++) {
-      const int j = begin + (i * kRowsThreads + threadIdx.x) * 4;
-      if (j >= end) continue;
-      double q[4];
-#pragma unroll
-      for (int k = 0; k < 4; k++) q[k] = j + k == label ? fma(v[4 * i + k], scale, -c) : v[4 * i + k] * scale;
-      if (j + 3 < end) {
-        *reinterpret_cast<double4v *>(r + j) = double4v{q[0], q[1], q[2], q[3]};
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-          if (j + k < end) r[j + k] = q[k];
-      }
-    }
-  }
-  if (CS > 1) cooperative_groups::this_cluster().sync();  // nobody leaves while its slots may be read
+  sum = warp_total(sum);
+  if (lane != 0) return;
+  row_loss[row] = keep ? -(z[row * pitch + label] - top - log(sum)) : 0.0;
+  row_stats[row] = keep ? make_double2(top, (gloss ? *gloss : 1.0) * inv_denom / sum) : make_double2(0.0, 0.0);
+  if (!keep && label != -1) atomicExch(status, 101);  // not a class and not "left out"
 }
 
-// The same for rows that eight CTAs cannot hold (over 65 536 classes): the running
-// maximum and sum of each thread in one pass, p in a second.
-template <bool GRAD>
-__global__ void __launch_bounds__(kRowsThreads)
-xent_long_rows_kernel(double *__restrict__ z, const int *__restrict__ labels, const double *__restrict__ gloss,
-                      double *__restrict__ row_loss, int V, size_t pitch, double inv_denom, int *status) {
-  __shared__ double smem32[32];
-  double *r = z + (size_t)blockIdx.x * pitch;
-  const int label = labels[blockIdx.x];
-  const bool keep = label >= 0 && label < V;
-  if (!keep) {
-    if (threadIdx.x == 0) {
-      if (label != -1) atomicExch(status, 101);
-      row_loss[blockIdx.x] = 0.0;
-    }
-    if (GRAD)
-      for (int j = threadIdx.x; j < V; j += kRowsThreads) r[j] = 0.0;
-    return;
-  }
-  double own = -INFINITY, sum = 0.0;
-  for (int j0 = threadIdx.x; j0 < V; j0 += 8 * kRowsThreads) {
-    double v[8], m = own;
-#pragma unroll
-    for (int k = 0; k < 8; k++) v[k] = j0 + k * kRowsThreads < V ? r[j0 + k * kRowsThreads] : -INFINITY;
-#pragma unroll
-    for (int k = 0; k < 8; k++) m = fmax(m, v[k]);
-    if (m > own) {
-      sum *= exp(own - m);
-      own = m;
-    }
-    // (own stays -inf while all classes so far have probability 0; a NaN enters the sum)
-#pragma unroll
-    for (int k = 0; k < 8; k++)
-      if (j0 + k * kRowsThreads < V) sum += v[k] == -INFINITY ? 0.0 : exp(v[k] - own);
-  }
-  const double top = block_reduce(own, true, smem32);
-  sum = block_reduce(own == -INFINITY && sum == 0.0 ? 0.0 : sum * exp(own - top), false, smem32);
-  if (threadIdx.x == 0) row_loss[blockIdx.x] = -(r[label] - top - log(sum));
-  if (GRAD) {
-    __syncthreads();
-    const double c = (gloss ? *gloss : 1.0) * inv_denom, scale = c / sum;
-    for (int j0 = threadIdx.x; j0 < V; j0 += 8 * kRowsThreads) {
-      double v[8];
-#pragma unroll
-      for (int k = 0; k < 8; k++) v[k] = j0 + k * kRowsThreads < V ? r[j0 + k * kRowsThreads] : 0.0;
-#pragma unroll
-      for (int k = 0; k < 8; k++) {
-        const int j = j0 + k * kRowsThreads;
-        if (j < V) r[j] = j == label ? fma(exp(v[k] - top), scale, -c) : exp(v[k] - top) * scale;
-      }
-    }
-  }
-}
+// z becomes p for 512 classes x `strip` rows per CTA; the classes' sums over these rows
+// go to parts[blockIdx.y][pitch] (or are not wanted: null).
+constexpr int kApplyRows = 64;  // most rows of a strip
 
-template <bool GRAD, int CS>
-static int launch_rows(double *z, const int *labels, const double *gloss, double *row_loss, size_t rows, size_t V,
-                       size_t pitch, double inv_denom) {
-  Context &c = ctx();
-  const size_t piece = ((V + CS - 1) / CS + 3) / 4 * 4;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(rows * CS));
-  cfg.blockDim = dim3(kRowsThreads);
-  cfg.stream = c.stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CS;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = CS > 1 ? 1 : 0;
-  MG_CUDA_TRY(cudaLaunchKernelEx(&cfg, xent_rows_kernel<GRAD, CS>, z, labels, gloss, row_loss, (int)V, pitch,
-                                 (int)piece, inv_denom, c.kernel_status));
-  MG_LAUNCH_CHECK("linear_xent rows");
-  return MG_OK;
-}
-
-template <bool GRAD>
-static int softmax_rows(double *z, const int *labels, const double *gloss, double *row_loss, size_t rows, size_t V,
-                        size_t pitch, double inv_denom) {
-  Context &c = ctx();
-  const size_t room = (size_t)kRowsThreads * kRowsValues;
-  if (V > 8 * room) {
-    xent_long_rows_kernel<GRAD><<<(unsigned)rows, kRowsThreads, 0, c.stream>>>(z, labels, gloss, row_loss, (int)V,
-                                                                             pitch, inv_denom, c.kernel_status);
-    MG_LAUNCH_CHECK("linear_xent rows");
-    return MG_OK;
+__global__ void __launch_bounds__(256)
+xent_apply_kernel(double *__restrict__ z, size_t pitch, size_t rows, int V, const double2 *__restrict__ row_stats,
+                  const int *__restrict__ labels, const double *__restrict__ gloss, double inv_denom,
+                  double *__restrict__ parts, int strip) {
+  __shared__ double2 stats[kApplyRows];
+  __shared__ int label[kApplyRows];
+  const size_t r0 = (size_t)blockIdx.y * strip;
+  const int count = rows - r0 < (size_t)strip ? (int)(rows - r0) : strip;
+  if ((int)threadIdx.x < count) {
+    stats[threadIdx.x] = row_stats[r0 + threadIdx.x];
+    label[threadIdx.x] = labels[r0 + threadIdx.x];
   }
-  // As few CTAs per row as hold it, more while that leaves SMs without any.
-  size_t cs = 1;
-  while (cs * (room - 4) < V && cs < 8) cs *= 2;
-  while (cs < 8 && rows * cs < (size_t)c.sm_count && V / cs > 2048) cs *= 2;
-  if (cs == 1) return launch_rows<GRAD, 1>(z, labels, gloss, row_loss, rows, V, pitch, inv_denom);
-  if (cs == 2) return launch_rows<GRAD, 2>(z, labels, gloss, row_loss, rows, V, pitch, inv_denom);
-  if (cs == 4) return launch_rows<GRAD, 4>(z, labels, gloss, row_loss, rows, V, pitch, inv_denom);
-  return launch_rows<GRAD, 8>(z, labels, gloss, row_loss, rows, V, pitch, inv_denom);
+  __syncthreads();
+  const int j = blockIdx.x * 512 + 2 * threadIdx.x;
+  if (j >= V) return;  // (the pair may reach into the pitch: what is there is not used)
+  const double c = (gloss ? *gloss : 1.0) * inv_denom;
+  double *at = z + r0 * pitch + j;
+  double s0 = 0.0, s1 = 0.0;
+#pragma unroll 4
+  for (int r = 0; r < count; r++, at += pitch) {
+    const double2 v = __ldcs(reinterpret_cast<const double2 *>(at)), st = stats[r];
+    // (scale 0 marks a row that is left out, whatever its logits are; a row whose sum is
+    // not finite has a NaN or 0 scale from it and exponentials to match)
+    const bool out = label[r] < 0 || label[r] >= V;
+    double p0 = out ? 0.0 : exp(v.x - st.x) * st.y, p1 = out ? 0.0 : exp(v.y - st.x) * st.y;
+    if (j == label[r]) p0 -= c;
+    if (j + 1 == label[r]) p1 -= c;
+    s0 += p0;
+    s1 += p1;
+    *reinterpret_cast<double2 *>(at) = make_double2(p0, p1);
+  }
+  if (parts) *reinterpret_cast<double2 *>(parts + blockIdx.y * pitch + j) = make_double2(s0, s1);
 }
 
 // loss[0] = sum of the rows' losses / denom, one CTA, fixed order.
 __global__ void __launch_bounds__(1024)
 xent_loss_kernel(const double *__restrict__ row_loss, size_t M, double inv_denom, double *loss) {
   __shared__ double smem32[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   double sum = 0.0;
   for (size_t i = threadIdx.x; i < M; i += 1024) sum += row_loss[i];
-  sum = block_reduce(sum, false, smem32);
-  if (threadIdx.x == 0) loss[0] = sum * inv_denom;
+  sum = warp_total(sum);
+  if (lane == 0) smem32[warp] = sum;
+  __syncthreads();
+  if (warp != 0) return;
+  sum = warp_total(smem32[lane]);
+  if (lane == 0) loss[0] = sum * inv_denom;
 }
 
 // out[v] (+)= sum over the rows of p[rows][pitch]: a CTA per 64 columns, its warps the
@@ -664,6 +576,15 @@ static int run_head(const Head &h) {
   };
   const size_t at_z = take(true, R * Vp), at_loss = take(true, h.M), at_x = take(copy_x, h.M * Kp);
   const size_t at_w = take(copy_w, h.K * Vp);
+  const unsigned segments = (unsigned)((h.V + kSegment - 1) / kSegment);
+  // Strips of 64 rows, fewer where that would leave SMs without a CTA (at least four: each
+  // strip costs a row of sums).
+  const size_t wide = (h.V + 511) / 512;
+  size_t strip = R * wide / ((size_t)c.sm_count * 2);
+  strip = strip > (size_t)kApplyRows ? kApplyRows : (strip < 4 ? 4 : strip);
+  const size_t strips = (R + strip - 1) / strip;
+  const size_t at_parts = take(true, 2 * R * segments), at_stats = take(true, 2 * R);
+  const size_t at_sums = take(h.grad && h.gbias, strips * Vp);
   double *ws = nullptr;
   int rc = mg_alloc(need, &ws);
   if (rc != MG_OK) return rc;
@@ -690,24 +611,33 @@ static int run_head(const Head &h) {
       fwd.ldb = ldw;
       fwd.ldd = Vp;
       if ((r = run_gemm_ext(fwd)) != MG_OK) return r;
-      r = h.grad ? softmax_rows<true>(z, h.labels + m0, h.gloss, ws + at_loss + m0, rows, h.V, Vp, inv)
-                 : softmax_rows<false>(z, h.labels + m0, h.gloss, ws + at_loss + m0, rows, h.V, Vp, inv);
-      if (r != MG_OK) return r;
+      double2 *parts = reinterpret_cast<double2 *>(ws + at_parts), *stats = reinterpret_cast<double2 *>(ws + at_stats);
+      const int *labels = h.labels + m0;
+      xent_segments_kernel<<<grid_for(rows * segments * 32, 256, 32), 256, 0, c.stream>>>(z, Vp, rows, (int)h.V, segments, parts);
+      MG_LAUNCH_CHECK("linear_xent segments");
+      xent_join_kernel<<<(unsigned)((rows * 32 + 255) / 256), 256, 0, c.stream>>>(
+          z, Vp, parts, segments, labels, h.gloss, rows, (int)h.V, inv, stats, ws + at_loss + m0, c.kernel_status);
+      MG_LAUNCH_CHECK("linear_xent join");
+      if (!h.grad) continue;
+      const unsigned used = (unsigned)((rows + strip - 1) / strip);
+      xent_apply_kernel<<<dim3((unsigned)wide, used), 256, 0, c.stream>>>(
+          z, Vp, rows, (int)h.V, stats, labels, h.gloss, inv, h.gbias ? ws + at_sums : nullptr, (int)strip);
+      MG_LAUNCH_CHECK("linear_xent apply");
       const bool first = m0 == 0;
-      if (h.grad && h.gx) {
+      if (h.gx) {
         GemmExt e{{z, w, h.gx + m0 * h.K, rows, h.K, h.V, true, true, !(h.flags & MG_ACC_STORE_A), MG_EPI_NONE, nullptr}};
         e.lda = Vp;
         e.ldb = ldw;
         if ((r = run_gemm_ext(e)) != MG_OK) return r;
       }
-      if (h.grad && h.gw) {
+      if (h.gw) {
         GemmExt e{{xb, z, h.gw, h.K, h.V, rows, false, false, !first || !(h.flags & MG_ACC_STORE_B), MG_EPI_NONE, nullptr}};
         e.lda = ldx;
         e.ldb = Vp;
         if ((r = run_gemm_ext(e)) != MG_OK) return r;
       }
-      if (h.grad && h.gbias) {
-        if ((r = column_sums(z, Vp, rows, h.V, h.gbias, !first || !(h.flags & MG_ACC_STORE_C))) != MG_OK) return r;
+      if (h.gbias) {
+        if ((r = column_sums(ws + at_sums, Vp, used, h.V, h.gbias, !first || !(h.flags & MG_ACC_STORE_C))) != MG_OK) return r;
       }
     }
     xent_loss_kernel<<<1, 1024, 0, c.stream>>>(ws + at_loss, h.M, inv, h.loss);
