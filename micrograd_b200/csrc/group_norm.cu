@@ -1009,16 +1009,21 @@ static int launch_warp(const TeamArgs &a, const TeamPlan &t) {
   return MG_OK;
 }
 
-// Walkers over the samples in the tile form: waves of the resident
-// CTAs times samples per walker, and half a sample for the first one's copies that
-// nothing overlaps, should be least.
-static size_t tile_walkers(const NormShape &s, const TeamPlan &t) {
-  // CTAs per SM: 64 registers per thread, 228 KB of shared memory (1 KB of it per CTA)
+// CTAs (clusters) of the tile form that are resident at once: 64 registers per thread,
+// 228 KB of shared memory per SM (1 KB of it per CTA).
+static size_t resident_ctas(const TeamPlan &t) {
   size_t per_sm = 1024 / (size_t)t.threads;
   const size_t by_smem = (228 << 10) / (t.smem + 2048);
   if (by_smem < per_sm) per_sm = by_smem;
-  size_t resident = (size_t)ctx().sm_count * (per_sm ? per_sm : 1) / t.cs;
-  if (resident < 1) resident = 1;
+  const size_t resident = (size_t)ctx().sm_count * (per_sm ? per_sm : 1) / t.cs;
+  return resident ? resident : 1;
+}
+
+// Walkers over the samples of the backward pass in the tile form: waves of the resident
+// CTAs times samples per walker, and half a sample for the first one's copies that
+// nothing overlaps, should be least.
+static size_t tile_walkers(const NormShape &s, const TeamPlan &t) {
+  const size_t resident = resident_ctas(t);
   size_t best = 1;
   double least = 0.0;
   for (size_t walk = 1; walk <= s.N; walk++) {  // samples per walker
@@ -1097,7 +1102,10 @@ static int one_pass_fwd(const double *x, const double *gamma, const double *beta
     nstep = (s.N + 4 * U - 1) / (4 * U);
     if (nstep < fill) nstep = fill < (s.N + U - 1) / U ? fill : (s.N + U - 1) / U;
   } else {
-    nstep = tile_walkers(s, t);
+    // The same for CTAs (128 x 784 x 256 in groups of 8: 105 us; 117 with one wave of them).
+    nstep = resident_ctas(t) / s.G;
+    if (nstep > s.N) nstep = s.N;
+    if (nstep < (s.N + 3) / 4) nstep = (s.N + 3) / 4;
   }
   const TeamArgs a{x, gamma, beta, nullptr, mean, rstd, y, nullptr, s.N, s.P, t.Pc, nstep, s.C, s.G, s.D,
                    s.D / t.vec, t.TY, t.logL, eps, 1.0 / ((double)s.P * s.D), false};

@@ -17,8 +17,9 @@
 
 namespace mg {
 
-// Logits held at a time.
+// Logits held at a time, and rows (launches over strips of them have 65 535 at most).
 constexpr size_t kBlockBytes = (size_t)1 << 30;
+constexpr size_t kBlockRows = (size_t)1 << 18;
 
 __device__ __forceinline__ double warp_max(double v) {
 #pragma unroll
@@ -564,8 +565,10 @@ static int run_head(const Head &h) {
   const size_t Kp = pitch16(h.K), Vp = pitch16(h.V);
   const bool copy_w = h.V % 2 != 0 || off_16_bytes(h.w);
   const bool copy_x = h.grad || h.K % 2 != 0 || off_16_bytes(h.x);
-  size_t R = kBlockBytes / sizeof(double) / Vp / 128 * 128;
-  if (R < 128) R = 128;
+  size_t R = kBlockBytes / sizeof(double) / Vp;
+  R = R >= 128 ? R / 128 * 128 : R / 16 * 16;  // whole tiles
+  if (R < 16) R = 16;
+  if (R > kBlockRows) R = kBlockRows;
   if (R > h.M) R = h.M;
 
   size_t need = 0;

@@ -30,99 +30,118 @@ __device__ __forceinline__ double q8_inverse(double top) { return top >= 1e-300 
 __device__ __forceinline__ int q8_code(double x, double inverse) {
   const int q = __double2loint(x * inverse + 6755399441055744.0);
   const int hi = __double2hiint(x), some = (hi << 1) | __double2loint(x);
-  return q != 0 || some == 0 ? q : (hi < 0 ? -1 : 1);
+  return q != 0 || some == 0 ? q : (hi >> 31) | 1;
 }
 
-// Reads and writes of VEC neighbouring values and codes.
-template <int VEC> __device__ __forceinline__ void load_values(const double *p, double (&v)[VEC]) {
-  if constexpr (VEC == 4) {
-    const double4v t = ld_stream_v4(reinterpret_cast<const double4v *>(p));
-    v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
-  } else if constexpr (VEC == 2) {
-    const double2 t = __ldcs(reinterpret_cast<const double2 *>(p));
-    v[0] = t.x; v[1] = t.y;
-  } else {
-    v[0] = __ldcs(p);
+// Row and block in it of the blocks b, b + step, ... without a division for each.
+struct BlockWalk {
+  size_t row, row_step;
+  unsigned block, block_step, nb;
+  __device__ __forceinline__ BlockWalk(size_t b, size_t step, unsigned per_row, bool flat) : nb(per_row) {
+    row = flat ? 0 : b / nb;
+    block = flat ? 0 : (unsigned)(b - row * nb);
+    row_step = flat ? 0 : step / nb;
+    block_step = flat ? 0 : (unsigned)(step - row_step * nb);
   }
-}
+  __device__ __forceinline__ void next() {
+    row += row_step;
+    block += block_step;
+    if (block >= nb) {
+      block -= nb;
+      row++;
+    }
+  }
+};
 
-// LANES lanes take a block, VEC neighbouring columns each, UN blocks at a time so that
-// 64 to 128 bytes per lane are on their way.  A lane of a block's ragged end has no
-// column; LANES x VEC = 64.
-template <int VEC, int UN, bool FLAT>
-__global__ void __launch_bounds__(kQ8Threads)
+// A warp per block, two columns per lane, UN blocks at a time so that 32 to 64 bytes per
+// lane are on their way.  The integer units bound this kernel before HBM does, so the
+// block's maximum is taken by two warp-wide integer reductions: of the high words of
+// |x|, then of the low words under the largest high word (their bit patterns are in the
+// order of the values, infinity and NaN above all numbers); and its two quotients are
+// taken by one lane, for all UN blocks at once.
+// PAIR: the columns are neighbours (even rows, aligned), else 32 apart.  FLAT: rows are
+// whole blocks.
+// 65 536 x 1024: 135 us with two blocks at a time and six CTAs per SM, 151 with four and
+// four, 170 with the maximum by shuffles.
+template <bool PAIR, int UN, bool FLAT>
+__global__ void __launch_bounds__(kQ8Threads, UN == 2 ? 6 : 4)
 q8_pack_kernel(const double *__restrict__ x, signed char *__restrict__ codes, double *__restrict__ scales,
                size_t blocks, size_t N, unsigned nb) {
-  constexpr int LANES = VEC == 4 ? 16 : 32, PER = 64 / LANES;  // columns per lane
-  const int lane = threadIdx.x % LANES;
-  const size_t teams = (size_t)gridDim.x * (kQ8Threads / LANES);
-  // (all lanes of a warp make the same number of rounds: they shuffle together)
-  const size_t first = ((size_t)blockIdx.x * kQ8Threads + threadIdx.x) / LANES, rounds = (blocks + teams * UN - 1) / (teams * UN);
-  for (size_t round = 0; round < rounds; round++) {
-    double v[UN][PER];
+  const int lane = threadIdx.x & 31;
+  const size_t warps = (size_t)gridDim.x * (kQ8Threads / 32);
+  size_t b0 = ((size_t)blockIdx.x * kQ8Threads + threadIdx.x) >> 5;
+  BlockWalk walk(b0, warps, nb, FLAT);
+  for (; b0 < blocks; b0 += warps * UN) {
+    double v0[UN], v1[UN];
     size_t at[UN];
-    int cols[UN];  // columns of this lane
+    int cols[UN];  // columns of the block (0: there is no such block)
+    // Loads are never conditional (a value merged with a default is waited for at the
+    // merge, one after the other): a column that does not exist reads the block's first
+    // value, or the array's, and is dropped below.
 #pragma unroll
     for (int u = 0; u < UN; u++) {
-      const size_t b = first + (round * UN + u) * teams;
+      const size_t b = b0 + u * warps;
       cols[u] = 0;
+      at[u] = 0;
       if (b < blocks) {
         if (FLAT) {
-          at[u] = b * 64 + lane * PER;
-          cols[u] = PER;
+          at[u] = b * 64;
+          cols[u] = 64;
         } else {
-          const size_t row = blocks >> 32 ? b / nb : (size_t)((unsigned)b / nb);
-          const size_t c = (b - row * nb) * 64 + lane * PER;
-          at[u] = row * N + c;
-          cols[u] = c < N ? (N - c < PER ? (int)(N - c) : PER) : 0;
+          const size_t c = (size_t)walk.block * 64;
+          at[u] = walk.row * N + c;
+          cols[u] = N - c < 64 ? (int)(N - c) : 64;
         }
       }
-#pragma unroll
-      for (int k = 0; k < PER; k++) v[u][k] = 0.0;
-      if constexpr (VEC == PER) {
-        if (cols[u] > 0) load_values<VEC>(x + at[u], v[u]);  // (N is a multiple of VEC)
+      if (!FLAT) walk.next();
+      if (PAIR) {
+        const double2 t = __ldcs(reinterpret_cast<const double2 *>(x + at[u] + (2 * lane < cols[u] ? 2 * lane : 0)));
+        v0[u] = t.x;
+        v1[u] = t.y;
       } else {
-#pragma unroll
-        for (int k = 0; k < PER; k++)
-          if (k < cols[u]) v[u][k] = __ldcs(x + at[u] + k);
+        v0[u] = __ldcs(x + at[u] + (lane < cols[u] ? lane : 0));
+        v1[u] = __ldcs(x + at[u] + (lane + 32 < cols[u] ? lane + 32 : 0));
       }
     }
+    unsigned top_hi[UN], top_lo[UN];
 #pragma unroll
     for (int u = 0; u < UN; u++) {
-      // NaN > infinity > every finite number in the order of the bit patterns of |x|.
-      unsigned long long m = 0;
+      // (a dropped column holds a value of the block, so it does not change the maximum)
+      const unsigned h0 = __double2hiint(v0[u]) & 0x7fffffff, h1 = __double2hiint(v1[u]) & 0x7fffffff;
+      top_hi[u] = __reduce_max_sync(0xffffffffu, h0 > h1 ? h0 : h1);
+      const unsigned l0 = h0 == top_hi[u] ? (unsigned)__double2loint(v0[u]) : 0u;
+      const unsigned l1 = h1 == top_hi[u] ? (unsigned)__double2loint(v1[u]) : 0u;
+      top_lo[u] = __reduce_max_sync(0xffffffffu, l0 > l1 ? l0 : l1);
+    }
+    unsigned my_hi = top_hi[0], my_lo = top_lo[0];
 #pragma unroll
-      for (int k = 0; k < PER; k++) {
-        const unsigned long long o = (unsigned long long)__double_as_longlong(fabs(v[u][k]));
-        m = o > m ? o : m;
-      }
+    for (int u = 1; u < UN; u++) {
+      my_hi = (lane & (UN - 1)) == u ? top_hi[u] : my_hi;
+      my_lo = (lane & (UN - 1)) == u ? top_lo[u] : my_lo;
+    }
+    const double top = __hiloint2double((int)my_hi, (int)my_lo);
+    const double my_inverse = my_hi < 0x7ff00000u ? q8_inverse(top) : 0.0;
+    if (lane < UN && b0 + lane * warps < blocks)
+      scales[b0 + lane * warps] = my_hi >= 0x7ff00000u ? __longlong_as_double(0x7ff8000000000000ll)
+                                  : my_inverse > 0.0   ? fmin(top / 127.0, kQ8MaxScale)
+                                                       : 0.0;
 #pragma unroll
-      for (int off = LANES / 2; off > 0; off >>= 1) {
-        const unsigned long long o = __shfl_xor_sync(0xffffffffu, m, off);
-        m = o > m ? o : m;
+    for (int u = 0; u < UN; u++) {
+      const double inverse = __shfl_sync(0xffffffffu, my_inverse, u);
+      double y0 = v0[u], y1 = v1[u];
+      if (top_hi[u] >= 0x7ff00000u) {  // (the same in the whole warp) an infinity or a NaN: signs
+        y0 = y0 > 0 ? 1.0 : (y0 < 0 ? -1.0 : 0.0);
+        y1 = y1 > 0 ? 1.0 : (y1 < 0 ? -1.0 : 0.0);
       }
-      const double top = __longlong_as_double((long long)m);
-      const bool finite = m < 0x7ff0000000000000ull;
-      const double inverse = finite ? q8_inverse(top) : 0.0;
-      unsigned word = 0;
-#pragma unroll
-      for (int k = 0; k < PER; k++) {
-        double y = v[u][k];
-        if (!finite) y = y > 0 ? 1.0 : (y < 0 ? -1.0 : 0.0);
-        word |= (unsigned)(q8_code(y, inverse) & 255) << (8 * k);
-      }
-      if (VEC == PER && cols[u] > 0) {
-        if (PER == 4) *reinterpret_cast<unsigned *>(codes + at[u]) = word;
-        else *reinterpret_cast<unsigned short *>(codes + at[u]) = (unsigned short)word;
+      const int q0 = q8_code(y0, inverse), q1 = q8_code(y1, inverse);
+      signed char *dst = codes + at[u];
+      if (PAIR) {
+        if (2 * lane < cols[u])
+          *reinterpret_cast<unsigned short *>(dst + 2 * lane) = (unsigned short)__byte_perm(q0, q1, 0x0040);
       } else {
-#pragma unroll
-        for (int k = 0; k < PER; k++)
-          if (k < cols[u]) codes[at[u] + k] = (signed char)(word >> (8 * k));
+        if (lane < cols[u]) dst[lane] = (signed char)q0;
+        if (lane + 32 < cols[u]) dst[lane + 32] = (signed char)q1;
       }
-      const size_t b = first + (round * UN + u) * teams;
-      if (lane == 0 && b < blocks)
-        scales[b] = !finite ? __longlong_as_double(0x7ff8000000000000ll)
-                            : inverse > 0.0 ? fmin(top / 127.0, kQ8MaxScale) : 0.0;
     }
   }
 }
@@ -134,7 +153,9 @@ q8_unpack_kernel(const signed char *__restrict__ codes, const double *__restrict
   constexpr int LANES = VEC == 4 ? 16 : 32, PER = 64 / LANES;
   const int lane = threadIdx.x % LANES;
   const size_t teams = (size_t)gridDim.x * (kQ8Threads / LANES);
-  for (size_t b0 = ((size_t)blockIdx.x * kQ8Threads + threadIdx.x) / LANES; b0 < blocks; b0 += teams * UN) {
+  size_t b0 = ((size_t)blockIdx.x * kQ8Threads + threadIdx.x) / LANES;
+  BlockWalk walk(b0, teams, nb, FLAT);
+  for (; b0 < blocks; b0 += teams * UN) {
     unsigned word[UN];
     double scale[UN];
     size_t at[UN], to[UN];
@@ -143,29 +164,30 @@ q8_unpack_kernel(const signed char *__restrict__ codes, const double *__restrict
     for (int u = 0; u < UN; u++) {
       const size_t b = b0 + u * teams;
       cols[u] = 0;
-      word[u] = 0;
+      at[u] = to[u] = 0;
       if (b < blocks) {
         if (FLAT) {
           at[u] = to[u] = b * 64 + lane * PER;
           cols[u] = PER;
         } else {
-          const size_t row = blocks >> 32 ? b / nb : (size_t)((unsigned)b / nb);
-          const size_t c = (b - row * nb) * 64 + lane * PER;
-          at[u] = row * N + c;
-          to[u] = row * pitch + c;
-          cols[u] = c < N ? (N - c < PER ? (int)(N - c) : PER) : 0;
+          const size_t c = (size_t)walk.block * 64 + lane * PER;
+          if (c < N) {
+            at[u] = walk.row * N + c;
+            to[u] = walk.row * pitch + c;
+            cols[u] = N - c < PER ? (int)(N - c) : PER;
+          }
         }
       }
-      if (cols[u] > 0) {
-        scale[u] = __ldg(scales + b);
-        if constexpr (VEC == PER) {
-          if (PER == 4) word[u] = __ldcs(reinterpret_cast<const unsigned *>(codes + at[u]));
-          else word[u] = __ldcs(reinterpret_cast<const unsigned short *>(codes + at[u]));
-        } else {
+      if (!FLAT) walk.next();
+      scale[u] = __ldg(scales + (b < blocks ? b : 0));
+      if constexpr (VEC == PER) {
+        if (PER == 4) word[u] = __ldcs(reinterpret_cast<const unsigned *>(codes + at[u]));
+        else word[u] = __ldcs(reinterpret_cast<const unsigned short *>(codes + at[u]));
+      } else {
+        word[u] = 0;
 #pragma unroll
-          for (int k = 0; k < PER; k++)
-            if (k < cols[u]) word[u] |= (unsigned)(unsigned char)codes[at[u] + k] << (8 * k);
-        }
+        for (int k = 0; k < PER; k++)
+          word[u] |= (unsigned)(unsigned char)codes[at[u] + (k < cols[u] ? k : 0)] << (8 * k);
       }
     }
 #pragma unroll
@@ -600,16 +622,14 @@ int mg_q8_pack(const double *x, signed char *codes, double *scales, size_t M, si
   if (M == 0 || N == 0) return MG_OK;
   const size_t nb = q8_blocks(N), blocks = M * nb;
   cudaStream_t stream = ctx().stream;
-  const int vec = q8_vec(x, codes, N);
-  const unsigned grid = grid_for(blocks * (vec == 4 ? 16 : 32), kQ8Threads, 64);
-  if (vec == 4 && N % 64 == 0)
-    q8_pack_kernel<4, 4, true><<<grid, kQ8Threads, 0, stream>>>(x, codes, scales, blocks, N, (unsigned)nb);
-  else if (vec == 4)
-    q8_pack_kernel<4, 2, false><<<grid, kQ8Threads, 0, stream>>>(x, codes, scales, blocks, N, (unsigned)nb);
-  else if (vec == 2)
-    q8_pack_kernel<2, 4, false><<<grid, kQ8Threads, 0, stream>>>(x, codes, scales, blocks, N, (unsigned)nb);
+  const unsigned grid = grid_for(blocks * 32, kQ8Threads, 64), wide = (unsigned)nb;
+  const bool pair = q8_vec(x, codes, N) >= 2;
+  if (pair && N % 64 == 0)
+    q8_pack_kernel<true, 2, true><<<grid, kQ8Threads, 0, stream>>>(x, codes, scales, blocks, N, wide);
+  else if (pair)
+    q8_pack_kernel<true, 4, false><<<grid, kQ8Threads, 0, stream>>>(x, codes, scales, blocks, N, wide);
   else
-    q8_pack_kernel<1, 4, false><<<grid, kQ8Threads, 0, stream>>>(x, codes, scales, blocks, N, (unsigned)nb);
+    q8_pack_kernel<false, 4, false><<<grid, kQ8Threads, 0, stream>>>(x, codes, scales, blocks, N, wide);
   MG_LAUNCH_CHECK("q8_pack");
   return MG_OK;
 }

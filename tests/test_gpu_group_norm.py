@@ -220,6 +220,34 @@ def test_equal_values_and_offset_pointers(abi):
     near(mean.numpy(), want[1].astype(LD), bound[1])
 
 
+@pytest.mark.parametrize("p,g,d", [(1, 16, 64), (500, 2, 20), (40000, 1, 3)])
+def test_offsets_beyond_32_bits(abi, p, g, d):
+    """2.2e9 values, in each of the forms: the last samples are what they are alone."""
+    c = g * d
+    n = 2 ** 31 // (p * c) + max(1, 6000000 // (p * c))
+    few = max(1, min(64, 200000 // (p * c)))
+    size, tail = n * p * c, few * p * c
+    x, y = abi.empty(size), abi.empty(size)
+    abi.mg_fill_uniform01(x.ptr, size, 9, 0)
+    mean, rstd = abi.empty(n * g), abi.empty(n * g)
+    abi.mg_group_norm_fwd(x.ptr, None, None, y.ptr, mean.ptr, rstd.ptr, n, p, c, g, 1e-5, K.ACT_SILU)
+    xt, yt = np.empty(tail), np.empty(tail)
+    abi.mg_download(xt.ctypes.data, x.offset(size - tail), tail)
+    abi.mg_download(yt.ctypes.data, y.offset(size - tail), tail)
+    ref, bound = forward(xt.reshape(few, p, g, d), np.ones(c), np.zeros(c), 1e-5, K.ACT_SILU)
+    near(yt, ref[0], bound[0])
+    # backward with x as the upstream gradient
+    gg, gb = abi.empty(c), abi.empty(c)
+    abi.mg_group_norm_bwd(x.ptr, None, None, mean.ptr, rstd.ptr, x.ptr, y.ptr, gg.ptr, gb.ptr, n, p, c, g, K.ACT_SILU, 7)
+    abi.mg_download(yt.ctypes.data, y.offset(size - tail), tail)
+    m, r = np.empty(few * g), np.empty(few * g)
+    abi.mg_download(m.ctypes.data, mean.offset((n - few) * g), few * g)
+    abi.mg_download(r.ctypes.data, rstd.offset((n - few) * g), few * g)
+    v = xt.reshape(few, p, g, d)
+    ref, bound = backward(v, np.ones(c), np.zeros(c), m.reshape(few, g), r.reshape(few, g), v, K.ACT_SILU)
+    near(yt, ref[0], bound[0])
+
+
 def test_empty(abi):
     keep = abi.array([3.0] * 8)
     for n, p in ((0, 5), (5, 0)):

@@ -247,6 +247,27 @@ def test_rows_in_several_blocks(abi):
     abi.mg_check_kernel_status()
 
 
+def test_many_rows_of_few_classes(abi):
+    """More rows than one block takes (262 144), three classes: every row's gradient from
+    the formula, and sums to the bounds' accuracy."""
+    m, k, v = 600001, 2, 3
+    rng, x, w, b, y = problem(m, k, v, 29)
+    z = x @ w + b
+    e = np.exp(z - z.max(axis=1, keepdims=True))
+    p = e / e.sum(axis=1, keepdims=True)
+    keep, at = y >= 0, np.where(y >= 0, y, 0)
+    loss = -(np.log(p[np.arange(m), at]) * keep).sum() / m
+    p[np.arange(m), at] -= 1
+    p *= keep[:, None] / m
+    got_loss, got = call(abi, x, w, b, y, float(m), 1.0, [np.zeros(t.shape) for t in (x, w, b)], STORE)
+    assert abs(got_loss - loss) <= 4 * m * U * loss
+    # per row: a few roundings of logits below 10 and probabilities below 1
+    assert np.abs(got[0] - p @ w.T).max() <= 200 * U / m
+    assert np.abs(got[1] - x.T @ p).max() <= 4 * m * U * (np.abs(x).T @ np.abs(p)).max()
+    assert np.abs(got[2] - p.sum(axis=0)).max() <= 4 * m * U * np.abs(p).sum(axis=0).max()
+    abi.mg_check_kernel_status()
+
+
 def test_empty(abi):
     loss, gw = abi.array([3.0]), abi.array([2.0] * 6)
     abi.mg_linear_xent_fwd(None, None, None, None, loss.ptr, 0, 2, 3, 1.0)

@@ -300,13 +300,19 @@ def test_the_step_recorded_and_replayed(api, abi):
     got = [step(api, x, y, layers, norm, opt).data()[0]]
     opt.step()
     alive = layers[0].forward(x).sum()  # an eager graph of the same leaves
+    outside = api.Tensor([m, 100], xs[0])
+    outside.keep_8bit()
+    outside_values = outside.data().copy()
     rec = api.RecordedStep()
     rec.begin()
     loss = step(api, x, y, layers, norm, opt)
     opt.step()
     with pytest.raises(RuntimeError, match="made before the recording"):
         x.keep_8bit()
+    with pytest.raises(RuntimeError, match="other side"):
+        outside.add(1.0)
     rec.end()
+    assert outside.kept_8bit() and np.array_equal(outside.data(), outside_values)
     for a, c in zip(xs[1:], ys[1:]):
         x.copy_from_host(a)
         y.copy_from_host(c)

@@ -201,6 +201,39 @@ def test_relu_backward(abi, n):
         assert np.array_equal(out.numpy(), g * (codes > 0) + (0 if flags else old))
 
 
+def test_offsets_beyond_32_bits(abi):
+    """2.2e9 values: the last rows are packed and read back like the first."""
+    m, n = 2 ** 31 // 1000 + 70000, 1000
+    x = abi.empty(m * n)
+    abi.mg_fill_uniform01(x.ptr, m * n, 3, 0)
+    codes, scales = abi.empty(m * n // 8 + 1), abi.empty(m * 16)
+    abi.mg_q8_pack(x.ptr, codes.ptr, scales.ptr, m, n)
+    rows = 64
+    tail = np.empty(rows * n)
+    abi.mg_download(tail.ctypes.data, x.offset((m - rows) * n), rows * n)
+    want = encode(tail.reshape(rows, n))
+    got = np.empty(rows * n // 8)
+    abi.mg_download(got.ctypes.data, codes.ptr + (m - rows) * n, rows * n // 8)
+    assert np.array_equal(got.view(np.int8).reshape(rows, n), want[0])
+    s = np.empty(rows * 16)
+    abi.mg_download(s.ctypes.data, scales.offset((m - rows) * 16), rows * 16)
+    assert np.array_equal(s.reshape(rows, 16), want[1])
+    abi.mg_fill(x.ptr, 0.0, m * n)
+    abi.mg_q8_unpack(codes.ptr, scales.ptr, x.ptr, m, n)
+    abi.mg_download(tail.ctypes.data, x.offset((m - rows) * n), rows * n)
+    assert np.array_equal(tail.reshape(rows, n), decode(*want))
+    # the ReLU mask and the two products read the codes there as well
+    g = abi.empty(m)
+    abi.mg_fill(g.ptr, 0.0, m)
+    abi.mg_fill(g.offset(m - 1), 1.0, 1)
+    dw, w, dx = abi.empty(n), abi.array(np.ones(n)), x
+    abi.mg_gemm_tn_q8(codes.ptr, scales.ptr, g.ptr, dw.ptr, m, 1, n, 0)
+    assert np.array_equal(dw.numpy(), decode(*want)[-1])
+    abi.mg_gemm_nt_q8(g.ptr, w.ptr, dx.ptr, m, 1, n, 0, codes.ptr)
+    abi.mg_download(tail.ctypes.data, dx.offset((m - rows) * n), rows * n)
+    assert np.array_equal(tail.reshape(rows, n)[-1], (want[0][-1] > 0) * 1.0) and not tail[:-n].any()
+
+
 def test_empty(abi):
     out = abi.array([4.0] * 6)
     for m, n in ((0, 5), (5, 0)):
