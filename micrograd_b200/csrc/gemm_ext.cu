@@ -74,6 +74,7 @@ static GemmPlan plan_ext(int M, int N, int K, int sms) {
 // take one CTA over 100 us and all SMs 4.
 __global__ void __launch_bounds__(256)
 fold_tiles_kernel(GemmEpilogue ep, const int2 *__restrict__ tiles, int tiles_n, int bm, int bn, int M, int N) {
+  cudaGridDependencySynchronize();
   __shared__ double part[8][33];
   const int2 info = tiles[blockIdx.y];
   if (info.y == 0) return;  // a whole tile: written by the kernel itself
@@ -226,8 +227,8 @@ int run_gemm_ext(const GemmExt &e) {
   else if (d.a_kcontig) rc = launch_layout_ext<true, true>(plan.tile, L);
   else rc = launch_layout_ext<false, false>(plan.tile, L);
   if (rc != MG_OK || !split || !fold_here) return rc;
-  fold_tiles_kernel<<<dim3((unsigned)(plan.bm * plan.bn / 32), (unsigned)(tiles_m * tiles_n)), 256, 0,
-                      c.stream>>>(ep, table->dev_tiles, tiles_n, plan.bm, plan.bn, M, N);
+  MG_CUDA_TRY(launch_overlapped(fold_tiles_kernel, dim3((unsigned)(plan.bm * plan.bn / 32), (unsigned)(tiles_m * tiles_n)),
+                                dim3(256), ep, table->dev_tiles, tiles_n, plan.bm, plan.bn, M, N));
   MG_LAUNCH_CHECK("gemm fold");
   return MG_OK;
 }

@@ -257,6 +257,7 @@ constexpr int kParamRows = 32;
 __global__ void __launch_bounds__(32 * kParamRows)
 gn_bwd_params_kernel(const double *__restrict__ parts, size_t rows, int C, double *ggamma, double *gbeta,
                      bool acc_gamma, bool acc_beta, double *__restrict__ joined) {
+  cudaGridDependencySynchronize();
   __shared__ double sums[2][kParamRows][33];
   const int tx = threadIdx.x, ty = threadIdx.y, c = blockIdx.x * 32 + tx;
   const size_t begin = rows * blockIdx.y / gridDim.y, end = rows * (blockIdx.y + 1) / gridDim.y;
@@ -292,19 +293,18 @@ static size_t param_layers(size_t rows) {
 
 // parts has room for param_layers(rows) more rows behind the `rows` it holds.
 static int sum_params(double *parts, size_t rows, int C, double *ggamma, double *gbeta, int flags) {
-  Context &c = ctx();
   const bool acc_gamma = !(flags & MG_ACC_STORE_B), acc_beta = !(flags & MG_ACC_STORE_C);
   const unsigned wide = (unsigned)((C + 31) / 32), layers = (unsigned)param_layers(rows);
   if (layers > 1) {
     double *joined = parts + rows * 2 * C;
-    gn_bwd_params_kernel<<<dim3(wide, layers), dim3(32, kParamRows), 0, c.stream>>>(parts, rows, C, nullptr, nullptr,
-                                                                                   false, false, joined);
+    MG_CUDA_TRY(launch_overlapped(gn_bwd_params_kernel, dim3(wide, layers), dim3(32, kParamRows), parts, rows, C, nullptr,
+                                  nullptr, false, false, joined));
     MG_LAUNCH_CHECK("group_norm parameter gradients");
     parts = joined;
     rows = layers;
   }
-  gn_bwd_params_kernel<<<wide, dim3(32, kParamRows), 0, c.stream>>>(parts, rows, C, ggamma, gbeta, acc_gamma, acc_beta,
-                                                                    nullptr);
+  MG_CUDA_TRY(launch_overlapped(gn_bwd_params_kernel, dim3(wide), dim3(32, kParamRows), parts, rows, C, ggamma, gbeta,
+                                acc_gamma, acc_beta, nullptr));
   MG_LAUNCH_CHECK("group_norm parameter gradients");
   return MG_OK;
 }

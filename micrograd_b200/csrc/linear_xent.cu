@@ -45,6 +45,7 @@ constexpr int kSegment = 512;  // classes per warp: 16 per lane
 __global__ void __launch_bounds__(256)
 xent_segments_kernel(const double *__restrict__ z, size_t pitch, size_t rows, int V, unsigned segments,
                      double2 *__restrict__ out) {
+  cudaGridDependencySynchronize();
   const int lane = threadIdx.x & 31;
   const size_t all = rows * segments;
   for (size_t at = ((size_t)blockIdx.x * 256 + threadIdx.x) >> 5; at < all; at += (size_t)gridDim.x * 8) {
@@ -82,6 +83,7 @@ __global__ void __launch_bounds__(256)
 xent_join_kernel(const double *__restrict__ z, size_t pitch, const double2 *__restrict__ parts, unsigned segments,
                  const int *__restrict__ labels, const double *__restrict__ gloss, size_t rows, int V,
                  double inv_denom, double2 *__restrict__ row_stats, double *__restrict__ row_loss, int *status) {
+  cudaGridDependencySynchronize();
   const int lane = threadIdx.x & 31;
   const size_t row = ((size_t)blockIdx.x * 256 + threadIdx.x) >> 5;
   if (row >= rows) return;
@@ -110,6 +112,7 @@ __global__ void __launch_bounds__(256)
 xent_apply_kernel(double *__restrict__ z, size_t pitch, size_t rows, int V, const double2 *__restrict__ row_stats,
                   const int *__restrict__ labels, const double *__restrict__ gloss, double inv_denom,
                   double *__restrict__ parts, int strip) {
+  cudaGridDependencySynchronize();
   __shared__ double2 stats[kApplyRows];
   __shared__ int label[kApplyRows];
   const size_t r0 = (size_t)blockIdx.y * strip;
@@ -143,6 +146,7 @@ xent_apply_kernel(double *__restrict__ z, size_t pitch, size_t rows, int V, cons
 // loss[0] = sum of the rows' losses / denom, one CTA, fixed order.
 __global__ void __launch_bounds__(1024)
 xent_loss_kernel(const double *__restrict__ row_loss, size_t M, double inv_denom, double *loss) {
+  cudaGridDependencySynchronize();
   __shared__ double smem32[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   double sum = 0.0;
@@ -160,6 +164,7 @@ xent_loss_kernel(const double *__restrict__ row_loss, size_t M, double inv_denom
 constexpr int kColWarps = 16;
 __global__ void __launch_bounds__(32 * kColWarps)
 column_sums_kernel(const double *__restrict__ p, size_t pitch, size_t rows, size_t V, double *out, bool accumulate) {
+  cudaGridDependencySynchronize();
   __shared__ double part[kColWarps][64];
   const int lane = threadIdx.x, warp = threadIdx.y;
   const size_t c0 = (size_t)blockIdx.x * 64 + 2 * lane;
@@ -185,7 +190,8 @@ column_sums_kernel(const double *__restrict__ p, size_t pitch, size_t rows, size
 }
 
 static int column_sums(const double *p, size_t pitch, size_t rows, size_t V, double *out, bool accumulate) {
-  column_sums_kernel<<<(unsigned)((V + 63) / 64), dim3(32, kColWarps), 0, ctx().stream>>>(p, pitch, rows, V, out, accumulate);
+  MG_CUDA_TRY(launch_overlapped(column_sums_kernel, dim3((unsigned)((V + 63) / 64)), dim3(32, kColWarps), p, pitch, rows,
+                                V, out, accumulate));
   MG_LAUNCH_CHECK("linear_xent column sums");
   return MG_OK;
 }
@@ -257,6 +263,11 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_fwd_kernel(const FewRows
   __shared__ bool is_last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, v0 = blockIdx.x * kSlab;
   const int c0 = v0 + few_class<PAIR>(lane, 0), c1 = v0 + few_class<PAIR>(lane, 1);
+  // (what the end needs, asked for now)
+  const int label = warp < a.M ? a.labels[warp] : -1;
+  double bias[2];
+#pragma unroll
+  for (int j = 0; j < 2; j++) bias[j] = a.bias && v0 + lane + 32 * j < a.V ? __ldg(a.bias + v0 + lane + 32 * j) : 0.0;
   double acc[MR][2];
 #pragma unroll
   for (int i = 0; i < MR; i++) acc[i][0] = acc[i][1] = 0.0;
@@ -295,7 +306,9 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_fwd_kernel(const FewRows
   }
   __syncthreads();
   // A warp per row: its 64 logits, two per lane.
-  for (int i = warp; i < a.M; i += kFewWarps) {
+  static_assert(kFewRows <= kFewWarps, "a warp per row");
+  if (warp < a.M) {
+    const int i = warp;
     double z[2];
 #pragma unroll
     for (int j = 0; j < 2; j++) {
@@ -305,10 +318,10 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_fwd_kernel(const FewRows
         double t = 0.0;
 #pragma unroll
         for (int w = 0; w < kFewWarps; w++) t += sums[w][i][s];
-        if (a.bias) t += a.bias[c];
+        t += bias[j];
         z[j] = t;
         if (a.grad) a.z[(size_t)i * a.Vp + c] = t;
-        if (c == a.labels[i]) a.at_label[i] = t;
+        if (c == label) a.at_label[i] = t;
       }
     }
     double top = fmax(z[0], z[1]);
@@ -326,14 +339,17 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_fwd_kernel(const FewRows
       out[1] = sum;
     }
   }
+  // (the gradients' kernel may be set up from here on; it waits for this one's end)
+  cudaTriggerProgrammaticLaunchCompletion();
   __threadfence();
   __syncthreads();
   if (threadIdx.x == 0) is_last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
   __syncthreads();
   if (!is_last) return;
   __threadfence();
-  for (int i = warp; i < a.M; i += kFewWarps) {
-    const bool keep = few_keep(a, i);
+  if (warp < a.M) {
+    const int i = warp;
+    const bool keep = label >= 0 && label < a.V;
     double top = -INFINITY;
     for (unsigned s = lane; s < gridDim.x; s += 32) top = fmax(top, __ldcg(a.slabs + ((size_t)s * a.M + i) * 2));
 #pragma unroll
@@ -349,7 +365,7 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_fwd_kernel(const FewRows
       a.rows[2 * i] = top;
       a.rows[2 * i + 1] = sum;
       red[i] = keep ? -(__ldcg(a.at_label + i) - top - log(sum)) : 0.0;
-      if (!keep && a.labels[i] != -1) atomicExch(a.status, 101);  // not a class and not "left out"
+      if (!keep && label != -1) atomicExch(a.status, 101);  // not a class and not "left out"
     }
   }
   __syncthreads();
@@ -389,9 +405,12 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_bwd_kernel(const FewRows
       x_next[r] = __ldg(a.x + (size_t)i * a.K + (k < a.K ? k : a.K - 1));
     }
   };
-  if (threadIdx.x < MR) kept[threadIdx.x] = few_keep(a, threadIdx.x);
+  // The inputs do not depend on the kernel before this one, which may still be running
+  // here; everything after the wait may.
   if (a.gx) fetch(0);
   if (a.K) fetch_x(0);
+  if (threadIdx.x < MR) kept[threadIdx.x] = few_keep(a, threadIdx.x);
+  cudaGridDependencySynchronize();
   __syncthreads();
   const double c = (a.gloss ? *a.gloss : 1.0) * a.inv_denom;
   for (int e = threadIdx.x; e < kSlab * MR; e += kFewThreads) {
@@ -417,6 +436,7 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_bwd_kernel(const FewRows
     p0[i] = ps[s0][i];
     p1[i] = ps[s1][i];
   }
+  cudaTriggerProgrammaticLaunchCompletion();
   for (int k0 = 0; k0 < a.K; k0 += kSlab) {
     const int ks = a.K - k0 < kSlab ? a.K - k0 : kSlab;
     __syncthreads();
@@ -491,6 +511,7 @@ few_rows_gx_kernel(const double *__restrict__ shares, unsigned slabs, size_t n, 
   __shared__ double part[16][17];
   const int e = threadIdx.x & 15, t = threadIdx.x >> 4;
   const size_t at = (size_t)blockIdx.x * 16 + e;
+  cudaGridDependencySynchronize();
   double s = 0.0;
   if (at < n) {
 #pragma unroll 8
@@ -512,12 +533,13 @@ template <int MR> static int launch_few(const FewRows &a, bool pair) {
   else few_rows_fwd_kernel<MR, false><<<slabs, kFewThreads, 0, c.stream>>>(a);
   MG_LAUNCH_CHECK("linear_xent (few rows)");
   if (!a.grad) return MG_OK;
-  if (pair) few_rows_bwd_kernel<MR, true><<<slabs, kFewThreads, 0, c.stream>>>(a);
-  else few_rows_bwd_kernel<MR, false><<<slabs, kFewThreads, 0, c.stream>>>(a);
+  MG_CUDA_TRY(launch_overlapped(pair ? few_rows_bwd_kernel<MR, true> : few_rows_bwd_kernel<MR, false>, dim3(slabs),
+                                dim3(kFewThreads), a));
   MG_LAUNCH_CHECK("linear_xent (few rows, gradients)");
   if (!a.gx) return MG_OK;
   const size_t n = (size_t)a.M * a.K;
-  few_rows_gx_kernel<<<(unsigned)((n + 15) / 16), 256, 0, c.stream>>>(a.shares, slabs, n, a.gx, a.acc_x);
+  MG_CUDA_TRY(launch_overlapped(few_rows_gx_kernel, dim3((unsigned)((n + 15) / 16)), dim3(256), a.shares, slabs, n,
+                                a.gx, a.acc_x));
   MG_LAUNCH_CHECK("linear_xent (few rows, gx)");
   return MG_OK;
 }
@@ -616,15 +638,17 @@ static int run_head(const Head &h) {
       if ((r = run_gemm_ext(fwd)) != MG_OK) return r;
       double2 *parts = reinterpret_cast<double2 *>(ws + at_parts), *stats = reinterpret_cast<double2 *>(ws + at_stats);
       const int *labels = h.labels + m0;
-      xent_segments_kernel<<<grid_for(rows * segments * 32, 256, 32), 256, 0, c.stream>>>(z, Vp, rows, (int)h.V, segments, parts);
+      MG_CUDA_TRY(launch_overlapped(xent_segments_kernel, dim3(grid_for(rows * segments * 32, 256, 32)), dim3(256), z, Vp,
+                                    rows, (int)h.V, segments, parts));
       MG_LAUNCH_CHECK("linear_xent segments");
-      xent_join_kernel<<<(unsigned)((rows * 32 + 255) / 256), 256, 0, c.stream>>>(
-          z, Vp, parts, segments, labels, h.gloss, rows, (int)h.V, inv, stats, ws + at_loss + m0, c.kernel_status);
+      MG_CUDA_TRY(launch_overlapped(xent_join_kernel, dim3((unsigned)((rows * 32 + 255) / 256)), dim3(256), z, Vp, parts,
+                                    segments, labels, h.gloss, rows, (int)h.V, inv, stats, ws + at_loss + m0,
+                                    c.kernel_status));
       MG_LAUNCH_CHECK("linear_xent join");
       if (!h.grad) continue;
       const unsigned used = (unsigned)((rows + strip - 1) / strip);
-      xent_apply_kernel<<<dim3((unsigned)wide, used), 256, 0, c.stream>>>(
-          z, Vp, rows, (int)h.V, stats, labels, h.gloss, inv, h.gbias ? ws + at_sums : nullptr, (int)strip);
+      MG_CUDA_TRY(launch_overlapped(xent_apply_kernel, dim3((unsigned)wide, used), dim3(256), z, Vp, rows, (int)h.V, stats,
+                                    labels, h.gloss, inv, h.gbias ? ws + at_sums : nullptr, (int)strip));
       MG_LAUNCH_CHECK("linear_xent apply");
       const bool first = m0 == 0;
       if (h.gx) {
@@ -643,7 +667,7 @@ static int run_head(const Head &h) {
         if ((r = column_sums(ws + at_sums, Vp, used, h.V, h.gbias, !first || !(h.flags & MG_ACC_STORE_C))) != MG_OK) return r;
       }
     }
-    xent_loss_kernel<<<1, 1024, 0, c.stream>>>(ws + at_loss, h.M, inv, h.loss);
+    MG_CUDA_TRY(launch_overlapped(xent_loss_kernel, dim3(1), dim3(1024), ws + at_loss, h.M, inv, h.loss));
     MG_LAUNCH_CHECK("linear_xent loss");
     return MG_OK;
   }();

@@ -526,6 +526,7 @@ q8_tall_kernel(const signed char *__restrict__ codes, const double *__restrict__
 
 __global__ void __launch_bounds__(256)
 q8_tall_join_kernel(const double *__restrict__ parts, size_t pieces, size_t n, double *dB, bool accumulate) {
+  cudaGridDependencySynchronize();
   const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= n) return;
   double s = 0.0;
@@ -562,7 +563,8 @@ static int launch_tall(const signed char *codes, const double *scales, const dou
     q8_tall_kernel<NN, kCodes1><<<grid, kTallThreads, 0, c.stream>>>(codes, scales, G, parts, M, (int)N, K, gx, piece);
   MG_LAUNCH_CHECK("gemm_tn_q8 (few columns)");
   if (direct) return MG_OK;
-  q8_tall_join_kernel<<<(unsigned)((K * N + 255) / 256), 256, 0, c.stream>>>(parts, pieces, K * N, dB, accumulate != 0);
+  MG_CUDA_TRY(launch_overlapped(q8_tall_join_kernel, dim3((unsigned)((K * N + 255) / 256)), dim3(256), parts, pieces, K * N,
+                                dB, accumulate != 0));
   MG_LAUNCH_CHECK("gemm_tn_q8 (join)");
   return mg_free(parts);
 }

@@ -270,11 +270,11 @@ def test_a_training_step_of_all_three(api, abi):
     abi.mg_check_kernel_status()
 
 
-def test_the_step_recorded_and_replayed(api, abi):
+@pytest.mark.parametrize("m", [48, 3, 1])
+def test_the_step_recorded_and_replayed(api, abi, m):
     """Replays give what the same steps give one launch at a time, bit for bit, also while
     another graph of the same parameters is alive."""
     rng, *_, layers, norm, params = model(api, 5)
-    m = 48
     opt = api.SGD(params, 0.05)
     start = [p.data().copy() for p in params]
     xs = [rng.standard_normal((m, 100)) for _ in range(4)]
