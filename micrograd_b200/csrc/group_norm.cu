@@ -519,6 +519,7 @@ template <int K> __device__ __forceinline__ void lanes_sum(double (&v)[K], int w
 template <int VEC, int U, int R, int ACT, bool BWD>
 __global__ void __launch_bounds__(kWarpFormThreads, BWD ? 2 : 4) gn_warp_kernel(const TeamArgs a) {
   __shared__ double chan[BWD ? 2 * VEC * kWarpFormThreads : 1];
+  cudaGridDependencySynchronize();
   const int width = 1 << a.logL, l = threadIdx.x & (width - 1), ty = l / a.Dv, tx = l - ty * a.Dv;
   const size_t team = ((size_t)blockIdx.x * kWarpFormThreads + threadIdx.x) >> a.logL;
   const size_t n0 = team / a.G;
@@ -762,6 +763,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) gn_tile_kernel(const TeamArgs
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ double red[2][kTileThreads / 32][K];
   __shared__ double slot[2][K];
+  cudaGridDependencySynchronize();
   const int ty = threadIdx.x / a.Dv, tx = threadIdx.x - ty * a.Dv;
   const size_t team = blockIdx.x / CS, n0 = team / a.G;
   const int g = (int)(team - n0 * a.G), rank = CS > 1 ? (int)(blockIdx.x % CS) : 0;
@@ -1004,7 +1006,7 @@ static TeamPlan plan_norm(const NormShape &s, uintptr_t address_bits, bool bwd) 
 template <int VEC, int U, int R, int ACT, bool BWD>
 static int launch_warp(const TeamArgs &a, const TeamPlan &t) {
   const size_t ctas = ((a.nstep * a.G << t.logL) + kWarpFormThreads - 1) / kWarpFormThreads;
-  gn_warp_kernel<VEC, U, R, ACT, BWD><<<(unsigned)ctas, kWarpFormThreads, 0, ctx().stream>>>(a);
+  MG_CUDA_TRY(launch_overlapped(gn_warp_kernel<VEC, U, R, ACT, BWD>, dim3((unsigned)ctas), dim3(kWarpFormThreads), a));
   MG_LAUNCH_CHECK("group_norm (warp form)");
   return MG_OK;
 }
@@ -1051,12 +1053,14 @@ static int launch_tile(const TeamArgs &a, const TeamPlan &t) {
   cfg.blockDim = dim3((unsigned)t.threads);
   cfg.dynamicSmemBytes = t.smem;
   cfg.stream = ctx().stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CS;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // as launch_overlapped
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = CS;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = CS > 1 ? 1 : 0;
+  cfg.numAttrs = CS > 1 ? 2 : 1;
   MG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a));
   MG_LAUNCH_CHECK("group_norm (tile form)");
   return MG_OK;

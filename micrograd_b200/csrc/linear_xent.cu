@@ -261,6 +261,7 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_fwd_kernel(const FewRows
   __shared__ double sums[kFewWarps][MR][kSlab];
   __shared__ double red[32];
   __shared__ bool is_last;
+  cudaGridDependencySynchronize();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, v0 = blockIdx.x * kSlab;
   const int c0 = v0 + few_class<PAIR>(lane, 0), c1 = v0 + few_class<PAIR>(lane, 1);
   // (what the end needs, asked for now)
@@ -527,10 +528,9 @@ few_rows_gx_kernel(const double *__restrict__ shares, unsigned slabs, size_t n, 
 }
 
 template <int MR> static int launch_few(const FewRows &a, bool pair) {
-  Context &c = ctx();
   const unsigned slabs = (unsigned)((a.V + kSlab - 1) / kSlab);
-  if (pair) few_rows_fwd_kernel<MR, true><<<slabs, kFewThreads, 0, c.stream>>>(a);
-  else few_rows_fwd_kernel<MR, false><<<slabs, kFewThreads, 0, c.stream>>>(a);
+  MG_CUDA_TRY(launch_overlapped(pair ? few_rows_fwd_kernel<MR, true> : few_rows_fwd_kernel<MR, false>, dim3(slabs),
+                                dim3(kFewThreads), a));
   MG_LAUNCH_CHECK("linear_xent (few rows)");
   if (!a.grad) return MG_OK;
   MG_CUDA_TRY(launch_overlapped(pair ? few_rows_bwd_kernel<MR, true> : few_rows_bwd_kernel<MR, false>, dim3(slabs),

@@ -67,6 +67,7 @@ template <bool PAIR, int UN, bool FLAT>
 __global__ void __launch_bounds__(kQ8Threads, UN == 2 ? 6 : 4)
 q8_pack_kernel(const double *__restrict__ x, signed char *__restrict__ codes, double *__restrict__ scales,
                size_t blocks, size_t N, unsigned nb) {
+  cudaGridDependencySynchronize();
   const int lane = threadIdx.x & 31;
   const size_t warps = (size_t)gridDim.x * (kQ8Threads / 32);
   size_t b0 = ((size_t)blockIdx.x * kQ8Threads + threadIdx.x) >> 5;
@@ -150,6 +151,7 @@ template <int VEC, int UN, bool FLAT>
 __global__ void __launch_bounds__(kQ8Threads)
 q8_unpack_kernel(const signed char *__restrict__ codes, const double *__restrict__ scales,
                  double *__restrict__ x, size_t pitch, size_t blocks, size_t N, unsigned nb) {
+  cudaGridDependencySynchronize();
   constexpr int LANES = VEC == 4 ? 16 : 32, PER = 64 / LANES;
   const int lane = threadIdx.x % LANES;
   const size_t teams = (size_t)gridDim.x * (kQ8Threads / LANES);
@@ -216,6 +218,7 @@ static size_t q8_blocks(size_t N) { return (N + kQ8Block - 1) / kQ8Block; }
 __global__ void __launch_bounds__(kQ8Threads)
 q8_relu_bwd_kernel(const signed char *__restrict__ codes, const double *g, double *gx, size_t n,
                    bool accumulate) {
+  cudaGridDependencySynchronize();
   const size_t stride = (size_t)gridDim.x * kQ8Threads;
   for (size_t i = (size_t)blockIdx.x * kQ8Threads + threadIdx.x; i < n; i += stride) {
     const double v = g[i] * (codes[i] > 0 ? 1.0 : 0.0);
@@ -590,13 +593,13 @@ static int unpack_rows(const signed char *codes, const double *scales, double *x
   if (pitch % 4 != 0 && vec == 4) vec = pitch % 2 == 0 ? 2 : 1;
   const unsigned grid = grid_for(blocks * (vec == 4 ? 16 : 32), kQ8Threads, 64);
   if (vec == 4 && N % 64 == 0 && pitch == N)
-    q8_unpack_kernel<4, 4, true><<<grid, kQ8Threads, 0, stream>>>(codes, scales, x, pitch, blocks, N, (unsigned)nb);
+    MG_CUDA_TRY(launch_overlapped(q8_unpack_kernel<4, 4, true>, dim3(grid), dim3(kQ8Threads), codes, scales, x, pitch, blocks, N, (unsigned)nb));
   else if (vec == 4)
-    q8_unpack_kernel<4, 2, false><<<grid, kQ8Threads, 0, stream>>>(codes, scales, x, pitch, blocks, N, (unsigned)nb);
+    MG_CUDA_TRY(launch_overlapped(q8_unpack_kernel<4, 2, false>, dim3(grid), dim3(kQ8Threads), codes, scales, x, pitch, blocks, N, (unsigned)nb));
   else if (vec == 2)
-    q8_unpack_kernel<2, 4, false><<<grid, kQ8Threads, 0, stream>>>(codes, scales, x, pitch, blocks, N, (unsigned)nb);
+    MG_CUDA_TRY(launch_overlapped(q8_unpack_kernel<2, 4, false>, dim3(grid), dim3(kQ8Threads), codes, scales, x, pitch, blocks, N, (unsigned)nb));
   else
-    q8_unpack_kernel<1, 4, false><<<grid, kQ8Threads, 0, stream>>>(codes, scales, x, pitch, blocks, N, (unsigned)nb);
+    MG_CUDA_TRY(launch_overlapped(q8_unpack_kernel<1, 4, false>, dim3(grid), dim3(kQ8Threads), codes, scales, x, pitch, blocks, N, (unsigned)nb));
   MG_LAUNCH_CHECK("q8_unpack");
   return MG_OK;
 }
@@ -627,11 +630,11 @@ int mg_q8_pack(const double *x, signed char *codes, double *scales, size_t M, si
   const unsigned grid = grid_for(blocks * 32, kQ8Threads, 64), wide = (unsigned)nb;
   const bool pair = q8_vec(x, codes, N) >= 2;
   if (pair && N % 64 == 0)
-    q8_pack_kernel<true, 2, true><<<grid, kQ8Threads, 0, stream>>>(x, codes, scales, blocks, N, wide);
+    MG_CUDA_TRY(launch_overlapped(q8_pack_kernel<true, 2, true>, dim3(grid), dim3(kQ8Threads), x, codes, scales, blocks, N, wide));
   else if (pair)
-    q8_pack_kernel<true, 4, false><<<grid, kQ8Threads, 0, stream>>>(x, codes, scales, blocks, N, wide);
+    MG_CUDA_TRY(launch_overlapped(q8_pack_kernel<true, 4, false>, dim3(grid), dim3(kQ8Threads), x, codes, scales, blocks, N, wide));
   else
-    q8_pack_kernel<false, 4, false><<<grid, kQ8Threads, 0, stream>>>(x, codes, scales, blocks, N, wide);
+    MG_CUDA_TRY(launch_overlapped(q8_pack_kernel<false, 4, false>, dim3(grid), dim3(kQ8Threads), x, codes, scales, blocks, N, wide));
   MG_LAUNCH_CHECK("q8_pack");
   return MG_OK;
 }
@@ -649,8 +652,8 @@ int mg_relu_bwd_q8(const signed char *codes, const double *g, double *gx, size_t
   if (n && (!codes || !g || !gx)) return fail(MG_ERR_INVALID, "mg_relu_bwd_q8: null pointer");
   MG_ENSURE_INIT();
   if (n == 0) return MG_OK;
-  q8_relu_bwd_kernel<<<grid_for(n, kQ8Threads, 64), kQ8Threads, 0, ctx().stream>>>(codes, g, gx, n,
-                                                                                !(flags & MG_ACC_STORE_A));
+  MG_CUDA_TRY(launch_overlapped(q8_relu_bwd_kernel, dim3(grid_for(n, kQ8Threads, 64)), dim3(kQ8Threads), codes, g, gx, n,
+                                !(flags & MG_ACC_STORE_A)));
   MG_LAUNCH_CHECK("relu_bwd_q8");
   return MG_OK;
 }
