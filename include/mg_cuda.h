@@ -242,7 +242,7 @@ int mg_softmax_xent_bwd(const double *logits, const int *labels, const double *g
  * gradient with respect to the loss, each destination may be NULL, and
  * MG_ACC_STORE_A / _B / _C say that gx / gw / gbias hold nothing yet.  The logits
  * exist for a block of rows at a time, in a workspace from the pool of mg_alloc (at
- * most 1 GiB or 16 rows).  Any K and V; odd ones, and arrays off a 16-byte boundary,
+ * most 1 GiB or 16 rows; with up to four rows, M/64 of w's size more for gx).  Any K and V; odd ones, and arrays off a 16-byte boundary,
  * are copied once into rows the tensor kernel can take. */
 int mg_linear_xent_fwd(const double *x, const double *w, const double *bias, const int *labels,
                        double *loss1, size_t M, size_t K, size_t V, double denom);

@@ -111,7 +111,8 @@ std::shared_ptr<Tensor> softmax_cross_entropy(const std::shared_ptr<Tensor> &log
 // computed in the forward pass, which has the block's logits at hand (three products
 // instead of the four that going through them again in the backward pass would take),
 // and kept for backward(); where neither the input nor the head's parameters require a
-// gradient only the loss is computed.  A row with label -1 is left out (a padded
+// gradient only the loss is computed (backward() throws std::logic_error for one that
+// came to require a gradient later).  A row with label -1 is left out (a padded
 // batch): it adds nothing to the loss or any gradient, whatever its values are; it does
 // count in the default divisor.
 std::shared_ptr<Tensor> linear_cross_entropy(const std::shared_ptr<Tensor> &input, Linear &head,

@@ -547,6 +547,11 @@ static std::shared_ptr<Tensor> linear_xent_node(const std::shared_ptr<Tensor> &i
     }
     const double *gl = Access::grad(self).device_read();
     for (int i = 0; i < 3; i++) {
+      if (!grads[i] && Access::requires_grad(*Access::children(self)[i])) {
+        throw std::logic_error("linear_cross_entropy: a tensor that requires a gradient did not when the loss was computed");
+      }
+    }
+    for (int i = 0; i < 3; i++) {
       Tensor &kid = *Access::children(self)[i];
       if (!grads[i] || !Access::requires_grad(kid)) {
         continue;

@@ -137,6 +137,18 @@ def test_linear_cross_entropy_node(api):
         api.linear_cross_entropy(api.Tensor([m, k + 1]), head, y)
 
 
+def test_a_gradient_required_after_the_loss_is_refused(api):
+    rng = np.random.default_rng(3)
+    head = linear(api, rng.standard_normal((12, 9)), rng.standard_normal((1, 9)))
+    x = api.Tensor([5, 12], rng.standard_normal((5, 12)))
+    x.set_requires_grad(False)
+    loss = api.linear_cross_entropy(x, head, np.arange(5))
+    x.set_requires_grad(True)
+    with pytest.raises(RuntimeError, match="did not when the loss was computed"):
+        loss.backward()
+    assert not np.any(head.weights().grad())
+
+
 def test_keep_8bit_values_and_uses(api):
     rng = np.random.default_rng(3)
     m, n = 37, 150
