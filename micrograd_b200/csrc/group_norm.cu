@@ -931,8 +931,8 @@ struct TeamPlan {
 };
 
 // Values of x a lane holds in the warp form.  65 536 x 1024 in groups of 64, forward:
-// 174 us (6.2 TB/s) with 8 and four CTAs per SM, 222 us with 16 and two; backward with
-// 4: 2 % slower.
+// 172 us (6.3 TB/s, the rate of a copy) with 8 and four CTAs per SM; 16 values and two
+// CTAs took 1.28 times as long, 4 values backward 1.02 times.
 constexpr int kWarpValues = 8;
 
 static int log2_ceil(size_t n) {
@@ -959,9 +959,10 @@ static TeamPlan plan_norm(const NormShape &s, uintptr_t address_bits, bool bwd) 
     return t;
   }
   // Backward, four channels' parameters and sums do not fit the registers that 28 warps
-  // per SM leave (16-byte cells, 512 threads: 153 us for 128 x 784 x 256 in groups of 8
-  // channels with SiLU; 32-byte cells, 256 threads: 198).  Forward, where less is kept,
-  // CTAs of 256 threads are better (105 us against 121 with 512).
+  // per SM leave (128 x 784 x 256 in groups of 8 channels with SiLU: 140 us with 16-byte
+  // cells and 512 threads, 4.4 TB/s; 32-byte cells and 256 threads took 1.3 times as long).
+  // Forward, where less is kept, CTAs of 256 threads are better (103 us; 512 threads: 1.15
+  // times as long).
   if (bwd && t.vec > 2) t.vec = 2;
   Dv = s.D / t.vec;
   if (Dv > (size_t)kTileThreads) return t;
@@ -969,7 +970,7 @@ static TeamPlan plan_norm(const NormShape &s, uintptr_t address_bits, bool bwd) 
   // Where there are groups for all SMs several times over: as many CTAs per SM as have
   // their groups in its shared memory, and 1024 threads among them, so that one's copies
   // and sums overlap another's arithmetic (33 x 197 positions, 30 groups of 5 channels,
-  // backward: 15 us instead of 20 with CTAs of 512 threads).
+  // backward, 11.8 us; CTAs of 512 threads took 1.3 times as long).
   if (s.N * s.G >= (size_t)ctx().sm_count * 2) {
     const size_t per_sm = (224 << 10) / (s.P * (size_t)s.D * (bwd ? 16 : 8) + 1024);
     size_t fit = per_sm > 1 ? (1024 / per_sm + 31) / 32 * 32 : max_threads;
@@ -1086,7 +1087,7 @@ template <bool BWD> static int run_form(const TeamArgs &a, const TeamPlan &t, in
 }
 
 // Samples a team of the warp form has in its registers at a time.
-static size_t samples_at_once(const TeamPlan &t, bool bwd) {
+static size_t samples_at_once(const TeamPlan &t) {
   if (t.form != kFormWarp || !t.small) return 1;
   const int most = kWarpValues / t.vec;
   return most < 8 ? most : 8;
@@ -1102,11 +1103,12 @@ static int one_pass_fwd(const double *x, const double *gamma, const double *beta
   if (t.form == kFormWarp) {
     // About four rounds per team, for which its parameters are loaded once; fewer where
     // that would leave SMs idle.
-    const size_t U = samples_at_once(t, false), fill = (size_t)ctx().sm_count * 4 * (kWarpFormThreads >> t.logL) / s.G;
+    const size_t U = samples_at_once(t), fill = (size_t)ctx().sm_count * 4 * (kWarpFormThreads >> t.logL) / s.G;
     nstep = (s.N + 4 * U - 1) / (4 * U);
     if (nstep < fill) nstep = fill < (s.N + U - 1) / U ? fill : (s.N + U - 1) / U;
   } else {
-    // The same for CTAs (128 x 784 x 256 in groups of 8: 105 us; 117 with one wave of them).
+    // The same for CTAs (128 x 784 x 256 in groups of 8: 103 us; one wave of them took
+    // 1.1 times as long).
     nstep = resident_ctas(t) / s.G;
     if (nstep > s.N) nstep = s.N;
     if (nstep < (s.N + 3) / 4) nstep = (s.N + 3) / 4;
@@ -1122,7 +1124,7 @@ static int one_pass_bwd(const double *x, const double *gamma, const double *beta
   Context &c = ctx();
   // Each of the nstep walkers over the samples leaves a row of sums per channel, so
   // there are no more of them than keep the SMs busy.
-  const size_t U = samples_at_once(t, true);
+  const size_t U = samples_at_once(t);
   size_t nstep;
   if (t.form == kFormWarp) {
     nstep = (size_t)c.sm_count * 2 * (kWarpFormThreads >> t.logL) / s.G;

@@ -201,6 +201,20 @@ def test_relu_backward(abi, n):
         assert np.array_equal(out.numpy(), g * (codes > 0) + (0 if flags else old))
 
 
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_relu_backward_off_the_vector_boundaries(abi, off):
+    rng = np.random.default_rng(off)
+    n = 1003
+    codes, g, old = rng.integers(-3, 4, n + off).astype(np.int8), rng.standard_normal(n), rng.standard_normal(n)
+    packed, dg, out = Packed(abi, 1, n + off, codes, np.zeros(1)), abi.array(g), abi.array(old)
+    abi.mg_relu_bwd_q8(packed.codes.ptr + off, dg.ptr, out.ptr, n, 0)
+    assert np.array_equal(out.numpy(), g * (codes[off:] > 0) + old)
+    shifted, kept = abi.array(np.concatenate([np.zeros(off), g])), abi.array(np.concatenate([np.zeros(off), old]))
+    abi.mg_relu_bwd_q8(packed.codes.ptr, shifted.ptr + 8 * off, kept.ptr + 8 * off, n, 0)
+    assert np.array_equal(kept.numpy()[off:], g * (codes[:n] > 0) + old)
+    assert not np.any(kept.numpy()[:off])
+
+
 def test_offsets_beyond_32_bits(abi):
     """2.2e9 values: the last rows are packed and read back like the first."""
     m, n = 2 ** 31 // 1000 + 70000, 1000
