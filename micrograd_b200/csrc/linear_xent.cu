@@ -208,7 +208,7 @@ struct Head {
 };
 
 // ---------------------------------------------------------------------------
-// Up to four rows (a single one in the per-sample loop): everything is a stream over w, so no
+// Up to four rows (a single one in the per-sample loop), eight for some losses alone: everything is a stream over w, so no
 // tile of the tensor kernel is worth filling.  A CTA takes a slab of 64 classes.
 //   1. z = x w + bias of the slab, each warp every eighth row of w, and the slab's
 //      (max, sum of exp) per row; the CTA that finishes last joins the slabs (in order)
@@ -217,7 +217,7 @@ struct Head {
 //   3. gx: the slabs' shares, in order.
 // Left-out rows count as zeros of x and p, whatever x holds.
 // ---------------------------------------------------------------------------
-constexpr int kFewRows = 4, kSlab = 64, kFewThreads = 256, kFewWarps = kFewThreads / 32, kFewK = 128;
+constexpr int kFewRows = 4, kFewRowsFwd = 8, kSlab = 64, kFewThreads = 256, kFewWarps = kFewThreads / 32, kFewK = 128;
 
 struct FewRows {
   const double *x, *w, *bias;
@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_fwd_kernel(const FewRows
   }
   __syncthreads();
   // A warp per row: its 64 logits, two per lane.
-  static_assert(kFewRows <= kFewWarps, "a warp per row");
+  static_assert(MR <= kFewWarps, "a warp per row");
   if (warp < a.M) {
     const int i = warp;
     double z[2];
@@ -527,12 +527,17 @@ few_rows_gx_kernel(const double *__restrict__ shares, unsigned slabs, size_t n, 
   }
 }
 
+template <int MR, bool PAIR> static int launch_few_fwd(const FewRows &a) {
+  const unsigned slabs = (unsigned)((a.V + kSlab - 1) / kSlab);
+  MG_CUDA_TRY(launch_overlapped(few_rows_fwd_kernel<MR, PAIR>, dim3(slabs), dim3(kFewThreads), a));
+  MG_LAUNCH_CHECK("linear_xent (few rows)");
+  return MG_OK;
+}
+
 template <int MR> static int launch_few(const FewRows &a, bool pair) {
   const unsigned slabs = (unsigned)((a.V + kSlab - 1) / kSlab);
-  MG_CUDA_TRY(launch_overlapped(pair ? few_rows_fwd_kernel<MR, true> : few_rows_fwd_kernel<MR, false>, dim3(slabs),
-                                dim3(kFewThreads), a));
-  MG_LAUNCH_CHECK("linear_xent (few rows)");
-  if (!a.grad) return MG_OK;
+  const int rc = pair ? launch_few_fwd<MR, true>(a) : launch_few_fwd<MR, false>(a);
+  if (rc != MG_OK || !a.grad) return rc;
   MG_CUDA_TRY(launch_overlapped(pair ? few_rows_bwd_kernel<MR, true> : few_rows_bwd_kernel<MR, false>, dim3(slabs),
                                 dim3(kFewThreads), a));
   MG_LAUNCH_CHECK("linear_xent (few rows, gradients)");
@@ -571,13 +576,20 @@ static int run_few_rows(const Head &h) {
   const bool pair = h.V % 2 == 0 && !off_16_bytes(h.w) && !(a.gw && off_16_bytes(a.gw));
   if (h.M == 1) rc = launch_few<1>(a, pair);
   else if (h.M == 2) rc = launch_few<2>(a, pair);
-  else rc = launch_few<4>(a, pair);
+  else if (h.M <= (size_t)kFewRows) rc = launch_few<kFewRows>(a, pair);
+  else rc = launch_few_fwd<kFewRowsFwd, false>(a);  // (neighbours cannot be paired there)
   const int freed = mg_free(ws);
   return rc != MG_OK ? rc : freed;
 }
 
 static int run_head(const Head &h) {
   if (h.M <= (size_t)kFewRows) return run_few_rows(h);
+  const bool copy_w = h.V % 2 != 0 || off_16_bytes(h.w);
+  // The loss alone of five to eight rows streams over w too where the tensor kernel would
+  // need a copy of it: 5 and 8 rows x 676 x 90 181 143 and 177 us instead of 310, 300 x
+  // 5001 13 and 15 instead of 26.  (90 182 classes, without the copy: 119 on the tensor
+  // kernel, 142 and 177 here.  Two groups of eight rows lose to the copy at 64 x 30 001.)
+  if (!h.grad && copy_w && h.M <= (size_t)kFewRowsFwd) return run_few_rows(h);
   Context &c = ctx();
   // The tensor kernel takes operand rows of an even number of doubles from 16-byte
   // boundaries.  x and w that do not come like that are copied into rows that do (M K
@@ -585,7 +597,6 @@ static int run_head(const Head &h) {
   // any case, the rows that are left out as zeros: whatever they hold, 0 times it is
   // not 0 in x^T p.
   const size_t Kp = pitch16(h.K), Vp = pitch16(h.V);
-  const bool copy_w = h.V % 2 != 0 || off_16_bytes(h.w);
   const bool copy_x = h.grad || h.K % 2 != 0 || off_16_bytes(h.x);
   size_t R = kBlockBytes / sizeof(double) / Vp;
   R = R >= 128 ? R / 128 * 128 : R / 16 * 16;  // whole tiles

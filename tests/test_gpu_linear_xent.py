@@ -120,6 +120,25 @@ def test_loss_and_gradients(abi, shape):
     abi.mg_check_kernel_status()
 
 
+@pytest.mark.parametrize("shift", [0, 1])
+@pytest.mark.parametrize("shape", [(5, 300, 5001), (6, 1, 63), (7, 129, 257), (8, 676, 4099), (8, 40, 130), (9, 40, 4099), (6, 5, 1)])
+def test_loss_alone_of_five_rows_and_more(abi, shape, shift):
+    m, k, v = shape
+    rng, x, w, b, y = problem(m, k, v, 31)
+    y[1], y[m - 1] = -1, v - 1
+    ref = reference(x, w, b, y, 3.0, 1.0)
+    x[1] = np.nan  # (left out)
+    flat = [abi.array(np.concatenate([np.zeros(shift), t.reshape(-1)])) for t in (x, w, b)]
+    dy, loss = abi.int_array(y), abi.empty(1)
+    for _ in range(2):
+        abi.mg_linear_xent_fwd(*(t.offset(shift) for t in flat), dy.ptr, loss.ptr, m, k, v, 3.0)
+        near("loss", loss.numpy()[0], *ref["loss"])
+    bare = reference(np.where(np.isnan(x), 0, x), w, 0 * b, y, 3.0, 1.0)
+    abi.mg_linear_xent_fwd(flat[0].offset(shift), flat[1].offset(shift), None, dy.ptr, loss.ptr, m, k, v, 3.0)
+    near("loss", loss.numpy()[0], *bare["loss"])
+    abi.mg_check_kernel_status()
+
+
 @pytest.mark.parametrize("shape", [(5, 32, 130), (40, 64, 1000), (130, 33, 257)])
 def test_each_gradient_alone_and_no_bias(abi, shape):
     m, k, v = shape
