@@ -51,20 +51,25 @@ __device__ __forceinline__ double cta_sum(double v, double *smem32) {
 }
 
 // 1 / (1 + exp(-z)) in about 26 fp64 instructions, against some 45 for the library's exp
-// and a division: these kernels have 45 (forward) to 68 (backward) per element before
-// the fp64 units, not HBM, bound them.  With a = |z| and -a = k ln 2 + r, |r| <= 0.35:
-// exp(-a) = 2^k exp(r), exp(r) by its Taylor series to r^13 / 13! (the rest is below
-// 2^-56); then n / (1 + exp(-a)) with n = 1 or exp(-a) by one Newton step on the
-// hardware's first guess and one correction of the quotient.  |z| above 700 counts as
-// 700: what is lost is below 1e-300.  NaN: the callers multiply by z.
+// and a division: these kernels have 45 (forward) to 68 (backward) per element.  With
+// a = |z| and -a = k ln 2 + r, |r| <= 0.35: exp(-a) = 2^k exp(r), exp(r) by its Taylor
+// series to r^13 / 13! (the rest is below 2^-56); then n / (1 + exp(-a)) with n = 1 or
+// exp(-a) by one Newton step on the hardware's first guess and one correction of the
+// quotient by its remainder.  ln 2 is taken in two parts, its first 40 binary places and
+// the rest, so that k times the first (k has ten bits) is exact.
+// From |z| = 708 on exp(-a) counts as 0 (2^k would not be a normal number), which takes at
+// most 2.4e-305 from a value z or a derivative formed with it.  It has to be 0 and
+// nothing that is left over: z may be anything up to the largest number.  z = -infinity
+// gives 0, and so NaN times z, as the definition does; NaN stays NaN in z.
 __device__ __forceinline__ double sigmoid_onepath(double z) {
   // (compared as integers: the fp64 units have enough to do)
-  const double a = (__double2hiint(z) & 0x7fffffff) < 0x4085e000 ? fabs(z) : 700.0;  // high word of 700.0
+  const bool in = (__double2hiint(z) & 0x7fffffff) < 0x40862000;  // high word of 708.0
+  const double a = in ? fabs(z) : 708.0;
   const double kMagic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
-  const double km = fma(a, -1.4426950408889634074, kMagic);
+  const double km = fma(a, -1.4426950408889634, kMagic);  // 1 / ln 2
   const double kd = km - kMagic;
-  double r = fma(kd, -6.93147180369123816490e-01, -a);
-  r = fma(kd, -1.90821492927058770002e-10, r);
+  double r = fma(kd, -0x1.62e42fefa4000p-1, -a);
+  r = fma(kd, 0x1.8432a1b0e2634p-43, r);  // (the first places are rounded up)
   double q = 1.0 / 6227020800.0;
   q = fma(q, r, 1.0 / 479001600.0);
   q = fma(q, r, 1.0 / 39916800.0);
@@ -78,7 +83,7 @@ __device__ __forceinline__ double sigmoid_onepath(double z) {
   q = fma(q, r, 1.0 / 6.0);
   q = fma(q, r, 0.5);
   const double p = fma(r * r, q, r);  // exp(r) - 1
-  const double s = __hiloint2double((__double2loint(km) + 1023) << 20, 0);  // 2^k, k in [-1010, 0]
+  const double s = __hiloint2double(in ? (__double2loint(km) + 1023) << 20 : 0, 0);  // 2^k, k in [-1021, 0], or 0
   const double e = fma(s, p, s), d = 1.0 + e, n = __double2hiint(z) < 0 ? e : 1.0;
   double y;
   asm("rcp.approx.ftz.f64 %0, %1;" : "=d"(y) : "d"(d));

@@ -1,0 +1,80 @@
+"""GPU: the operators for larger models at the edges of what they accept."""
+import numpy as np
+import pytest
+
+from micrograd_b200 import cabi as K
+from test_gpu_group_norm import call_fwd, near
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -53
+LD = np.longdouble
+STORE = K.ACC_STORE_A | K.ACC_STORE_B | K.ACC_STORE_C
+MAX = np.finfo(np.float64).max
+
+
+def silu(z):
+    """z / (1 + exp(-z)) and its derivative in extended precision."""
+    z = z.astype(LD)
+    with np.errstate(all="ignore"):
+        e = np.exp(-z)
+        s = 1 / (1 + e)
+        return z / (1 + e), s * (1 + z * (1 - s))
+
+
+# Channel counts that take the warp form, the tile form and the general form.
+FORMS = {"warp": (3, 1, 8), "tile": (2, 40, 40), "general": (2, 1, 4200)}
+
+
+def silu_of(abi, form, z):
+    """silu(z) and silu'(z) as group norm computes them for the channels' values z: with
+    gamma = 0 a channel's z is its beta, and with one sample's gy = 1 at one position, and 0
+    elsewhere, gbeta is the derivative."""
+    n, p, c = FORMS[form]
+    ys, slopes = [], []
+    for at in range(0, len(z), c):
+        beta = np.zeros(c)
+        part = z[at:at + c]
+        beta[:len(part)] = part
+        x = np.random.default_rng(at).standard_normal((n, p, 1, c))
+        y, mean, rstd = call_fwd(abi, x, np.zeros(c), beta, 1e-5, K.ACT_SILU)
+        y = y.reshape(n * p, c)
+        assert all(np.array_equal(row, y[0], equal_nan=True) for row in y)
+        gy = np.zeros((n * p, c))
+        gy[-1] = 1.0
+        dev = [abi.array(v) for v in (x, np.zeros(c), beta, mean, rstd, gy)]
+        gx, gg, gb = abi.empty(x.size), abi.empty(c), abi.empty(c)
+        abi.mg_group_norm_bwd(*(v.ptr for v in dev), gx.ptr, gg.ptr, gb.ptr, n, p, c, 1, K.ACT_SILU, STORE)
+        if np.all(np.isfinite(part)):
+            assert not np.any(gx.numpy())
+        ys.append(y[0][:len(part)])
+        slopes.append(gb.numpy()[:len(part)])
+    return np.concatenate(ys), np.concatenate(slopes)
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+def test_silu_far_out(abi, form):
+    """The bounds: the sigmoid is good to 8 u where exp(z) is a normal number, and counts as
+    0 below exp(-708) = 3.3e-308: at most 745 * 3.3e-308 of a value or a derivative is lost
+    there, and nothing above 2^-1074 further out.  The derivative is s (1 + z (1 - s)): with s
+    off by 8 u s, 1 - s is off by 8 u s and what it is multiplied to by 8 u s |z|, so that with
+    the three roundings the derivative is good to 24 u s (1 + |z|), also where 1 - s is small."""
+    out = np.array([30, 600, 699.9999, 700, 705, 707.9, 708, 709, 709.8, 745, 746, 1e4, 1e10, 1e300, MAX])
+    z = np.concatenate([[0.0, 1e-300], out, -out])
+    y, slope = silu_of(abi, form, z)
+    ref, dref = silu(z)
+    near(y, ref, 10 * U * np.abs(ref) + 745 * 3.4e-308)
+    far = np.minimum(np.abs(z), 746.0)
+    near(slope, dref, 24 * U * (1 + far) / (1 + np.exp(np.minimum(-z, 700.0))) + 746 * 3.4e-308)
+    y, slope = silu_of(abi, form, np.array([np.inf, -np.inf, np.nan]))
+    assert y[0] == np.inf and np.all(np.isnan(y[1:])) and np.all(np.isnan(slope))
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+def test_silu_over_its_range(abi, form):
+    rng = np.random.default_rng(5)
+    z = np.concatenate([rng.uniform(-708, 708, 150), rng.standard_normal(150) * 4, rng.standard_normal(60) * 1e-8])
+    y, slope = silu_of(abi, form, z)
+    ref, dref = silu(z)
+    near(y, ref, 10 * U * np.abs(ref))
+    s = 1 / (1 + np.exp(-z.astype(LD)))
+    near(slope, dref, 24 * U * s * (1 + np.abs(z)))
