@@ -275,7 +275,8 @@ int mg_group_norm_bwd(const double *x, const double *gamma, const double *beta,
 /* ---- activations kept in 8 bits (no counterpart in the reference) --------- */
 /* x[M,N] becomes codes[M,N] (one byte each) and scales[M, ceil(N / MG_Q8_BLOCK)]: a
  * block of MG_Q8_BLOCK columns of a row shares scale = max |x| / 127, and
- * code = rint(x / scale), except that a value that is not 0 never gets code 0.  The
+ * code = rint(x * (127 / max |x|)) (the quotient and the product each rounded, ties to
+ * even), except that a value that is not 0 never gets code 0.  The
  * value kept is code * scale: at most scale away from x, at most scale / 2 where
  * |x| >= scale / 2; and the sign of the code is always the sign of x, so a ReLU mask
  * taken from the codes is exact.  A block whose largest magnitude is below 1e-300 is

@@ -4,7 +4,9 @@
 // may be shorter).  With a = max |x| over a block:
 //
 //   scale = a / 127,  code = rint(x (127 / a)),  and code = sign(x) where that
-//   rounds to 0 and x is not 0;  the value kept is code * scale.
+//   rounds to 0 and x is not 0;  the value kept is code * scale
+//
+// with each quotient and product rounded to fp64 before it is used.
 //
 // So a code is at most half a step from x (up to a whole step where a small value is
 // kept away from 0), and sign(code) = sign(x) always: a ReLU mask taken from the
@@ -26,9 +28,11 @@ static_assert(kQ8Block == 64, "the kernels deal a block to 16 or 32 lanes");
 __device__ __forceinline__ double q8_inverse(double top) { return top >= 1e-300 ? 127.0 / top : 0.0; }
 
 // rint(x * inverse), |x * inverse| < 128, as the low word of the sum with 1.5 * 2^52
-// (ties to even, like rint); the sign of x where that is 0 and x is not.
+// (ties to even, like rint); the sign of x where that is 0 and x is not.  The product is
+// rounded before the sum: one fma would give 63 for 2.5 under a maximum of 5, where
+// 2.5 (127 / 5) rounds to 63.5 and so to 64.
 __device__ __forceinline__ int q8_code(double x, double inverse) {
-  const int q = __double2loint(x * inverse + 6755399441055744.0);
+  const int q = __double2loint(__dadd_rn(__dmul_rn(x, inverse), 6755399441055744.0));
   const int hi = __double2hiint(x), some = (hi << 1) | __double2loint(x);
   return q != 0 || some == 0 ? q : (hi >> 31) | 1;
 }
@@ -61,7 +65,7 @@ struct BlockWalk {
 // taken by one lane, for all UN blocks at once.
 // PAIR: the columns are neighbours (even rows, aligned), else 32 apart.  FLAT: rows are
 // whole blocks.
-// 65 536 x 1024: 133 us with two blocks at a time and six CTAs per SM, 151 with four and
+// 65 536 x 1024: 134 us with two blocks at a time and six CTAs per SM, 151 with four and
 // four, 170 with the maximum by shuffles.
 template <bool PAIR, int UN, bool FLAT>
 __global__ void __launch_bounds__(kQ8Threads, UN == 2 ? 6 : 4)

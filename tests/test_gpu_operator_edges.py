@@ -4,6 +4,7 @@ import pytest
 
 from micrograd_b200 import cabi as K
 from test_gpu_group_norm import call_fwd, near
+from test_gpu_q8 import Packed, encode
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -53
@@ -78,3 +79,23 @@ def test_silu_over_its_range(abi, form):
     near(y, ref, 10 * U * np.abs(ref))
     s = 1 / (1 + np.exp(-z.astype(LD)))
     near(slope, dref, 24 * U * s * (1 + np.abs(z)))
+
+
+@pytest.mark.parametrize("n", [64, 66, 65, 127])
+def test_codes_between_two_steps(abi, n):
+    """Values at or beside half a step, where one rounding more or less is another code:
+    whole and half numbers under whole maxima, so that x (127 / max) is exactly a half or
+    next to one."""
+    rng = np.random.default_rng(n)
+    m = 600
+    top = np.concatenate([[5, 7, 9, 10, 3, 1], rng.integers(1, 2000, m - 6)]).astype(np.float64)[:, None]
+    x = np.rint(rng.uniform(-1, 1, (m, n)) * 2 * top) / 2
+    for c in range(0, n, 64):  # every block has its maximum and both of its halves
+        x[:, c] = top[:, 0]
+        if c + 2 < n:
+            x[:, c + 1], x[:, c + 2] = top[:, 0] / 2, -top[:, 0] / 2
+    want_codes, want_scales = encode(x)
+    dx, packed = abi.array(x), Packed(abi, m, n)
+    abi.mg_q8_pack(dx.ptr, packed.codes.ptr, packed.scales.ptr, m, n)
+    codes, scales = packed.read()
+    assert np.array_equal(codes, want_codes) and np.array_equal(scales, want_scales)
