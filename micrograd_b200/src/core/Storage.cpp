@@ -95,9 +95,7 @@ void Storage::pack8(size_t rows, size_t cols) {
   double *fp64 = dev_;
   dev_ = nullptr;
   dev_valid_ = false;
-  host_valid_ = false;
-  host_.clear();
-  host_.shrink_to_fit();
+  host_valid_ = false;  // (the vector keeps its size: data() may have lent it)
   check(mg_free(fp64), "free");
 }
 

@@ -68,6 +68,32 @@ TEST(ApiTest, MutableHostViews) {
   EXPECT_EQ(x->size(), static_cast<size_t>(3));
 }
 
+// A vector that data() has lent keeps its size through keep_8bit(), and says again what
+// the tensor holds once data() has been asked for again.
+TEST(ApiTest, LentViewsKeepTheirSizeThroughKeep8bit) {
+  std::vector<double> values(140);
+  for (size_t i = 0; i < values.size(); i++) values[i] = std::fmod(static_cast<double>(i) * 0.37, 1.0) - 0.5;
+  auto x = make({2, 70}, values);
+  std::vector<double> &lent = x->data();
+  lent[3] = 0.25;
+  x->keep_8bit();
+  EXPECT_EQ(lent.size(), static_cast<size_t>(140));
+  auto y = make({2, 70}, values);
+  const std::vector<double> &view = static_cast<const Tensor &>(*y).data();
+  y->keep_8bit();
+  EXPECT_EQ(view.size(), static_cast<size_t>(140));
+  EXPECT_EQ(&x->data(), &lent);
+  EXPECT_NEAR(lent[3], 0.25, 0.5 / 127 / 2 + 1e-15);
+  for (size_t i = 0; i < 140; i++) {
+    EXPECT_NEAR(static_cast<const Tensor &>(*y).data()[i], values[i], 0.5 / 127 + 1e-15);
+  }
+  // an element written through the lent reference, as after any other use
+  x->data();
+  lent[5] = 3.0;
+  EXPECT_NEAR(x->mul(2.0)->data()[5], 6.0, 0.0);
+  EXPECT_EQ(x->kept_8bit(), false);
+}
+
 // Linear::forward for a batch (the reference's forward only works for batch 1),
 // softmax cross-entropy, SGD: loss decreases and a step equals p - lr*g.
 TEST(ApiTest, BatchedLinearTrainingStep) {
