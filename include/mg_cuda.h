@@ -323,6 +323,7 @@ int mg_sgd_step_multi(double *const *params, const double *const *grads, const s
 int mg_graph_begin(void);
 int mg_graph_end(int *out_id);
 int mg_graph_recording(void); /* 1 between mg_graph_begin() and mg_graph_end() */
+int mg_graph_count(void);     /* recorded steps that exist: ended and not destroyed */
 int mg_graph_launch(int id);  /* enqueues the whole recorded step on the compute stream */
 int mg_graph_kernels(int id); /* kernel launches the recorded step contains (0 if unknown id) */
 int mg_graph_destroy(int id);

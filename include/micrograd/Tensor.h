@@ -106,7 +106,8 @@ public:
   // value), read the codes themselves; any other use makes an fp64 form of them again,
   // any write to the tensor ends the 8-bit form.  Refused (std::logic_error) for tensors
   // whose values share a buffer (parameters after SGD::enable_allreduce, load_mnist
-  // samples), and, while a step is recorded, for tensors made before the recording.
+  // samples), for tensors that a recorded step has used (its replays use the buffer where
+  // it was; until no recorded step is left), and, while a step is recorded, for tensors made before the recording.
   void keep_8bit();
   bool kept_8bit() const;
   // Read-only host views.  Unlike the mutable data()/grad() of the reference

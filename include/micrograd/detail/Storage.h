@@ -94,6 +94,7 @@ private:
   void sync_device_from_host();
   void sync_host_from_device();
   void drop_codes();     // the contents are about to be replaced
+  void note_step();      // a pointer to dev_ is handed out
   void expand();         // dev_ from the codes
   void download(double *values, size_t first, size_t n);  // current device contents, from either form
   bool fetch_mirror(double *value);  // true: *value is the mirrored, still current element
@@ -116,6 +117,7 @@ private:
   size_t code_rows_ = 0, code_cols_ = 0;
   bool dev_recorded_ = false;     // dev_ was allocated while a step was being recorded
   bool codes_recorded_ = false;
+  bool dev_in_step_ = false;      // a recorded step uses dev_, which was there before it
   std::vector<double> host_;
 };
 

@@ -97,6 +97,7 @@ SIGNATURES = {
     "mg_graph_begin": (C.c_int, []),
     "mg_graph_end": (C.c_int, [_ip]),
     "mg_graph_recording": (C.c_int, []),
+    "mg_graph_count": (C.c_int, []),
     "mg_graph_launch": (C.c_int, [C.c_int]),
     "mg_graph_kernels": (C.c_int, [C.c_int]),
     "mg_graph_destroy": (C.c_int, [C.c_int]),
@@ -133,7 +134,7 @@ SIGNATURES = {
 
 # Entry points whose int result is a value, not a status.
 _VALUE_INT = {"mg_device", "mg_sm_count", "mg_comm_rank", "mg_comm_world", "mg_comm_peer_path",
-              "mg_graph_kernels", "mg_graph_recording"}
+              "mg_graph_kernels", "mg_graph_recording", "mg_graph_count"}
 
 
 def declared_in_header(header_text: str) -> list[str]:

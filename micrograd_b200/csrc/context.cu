@@ -557,6 +557,12 @@ int mg_graph_end(int *out_id) {
 
 int mg_graph_recording(void) { return g_ctx.capturing ? 1 : 0; }
 
+int mg_graph_count(void) {
+  int count = 0;
+  for (const auto &step : g_steps) count += step.exec ? 1 : 0;
+  return count;
+}
+
 int mg_graph_launch(int id) {
   MG_ENSURE_INIT();
   MG_NOT_WHILE_RECORDING("mg_graph_launch");

@@ -49,6 +49,13 @@ void Storage::drop_codes() {
   }
 }
 
+// Replays of a step that is being recorded will use the buffer at the address it has now.
+void Storage::note_step() {
+  if (!dev_recorded_ && mg_graph_recording()) {
+    dev_in_step_ = true;
+  }
+}
+
 void Storage::pack8(size_t rows, size_t cols) {
   if (zero_ || size_ == 0) {
     return;  // nothing to keep
@@ -57,9 +64,13 @@ void Storage::pack8(size_t rows, size_t cols) {
     throw std::logic_error("keep_8bit: the values live in a buffer shared with other tensors");
   }
   const bool recording = mg_graph_recording() != 0;
+  if (dev_in_step_ && mg_graph_count() == 0) {
+    dev_in_step_ = false;  // the steps that used the buffer are gone
+  }
   if (codes_) {
-    // Kept in 8 bits already; an fp64 form that was made of them since goes again.
-    if (dev_ && recording == dev_recorded_) {
+    // Kept in 8 bits already; an fp64 form that was made of them since goes again, unless
+    // a recorded step reads it.
+    if (dev_ && recording == dev_recorded_ && !dev_in_step_) {
       double *fp64 = dev_;
       dev_ = nullptr;
       dev_valid_ = false;
@@ -67,12 +78,15 @@ void Storage::pack8(size_t rows, size_t cols) {
     }
     return;
   }
-  device_read();  // settles a pending upload, refreshes the device copy from a lent host view
-  if (recording != dev_recorded_) {
+  if (dev_ && recording != dev_recorded_) {
     throw std::logic_error(recording
                                ? "keep_8bit: a tensor made before the recording keeps its buffer while a step is recorded"
                                : "keep_8bit: a tensor made by a recorded step keeps its buffer");
   }
+  if (dev_in_step_) {
+    throw std::logic_error("keep_8bit: a recorded step uses the tensor's buffer");
+  }
+  device_read();  // settles a pending upload, refreshes the device copy from a lent host view
   const size_t blocks = (cols + MG_Q8_BLOCK - 1) / MG_Q8_BLOCK;
   signed char *codes = nullptr;
   double *scales = nullptr;
@@ -138,6 +152,7 @@ void Storage::ensure_device_buffer() {
     check(mg_alloc(size_, &dev_), "device allocation");
     owns_dev_ = true;
     dev_recorded_ = mg_graph_recording() != 0;
+    dev_in_step_ = false;
   }
 }
 
@@ -239,6 +254,7 @@ const double *Storage::device_read() {
   } else if (!dev_valid_) {
     sync_device_from_host();
   }
+  note_step();
   return dev_;
 }
 
@@ -247,6 +263,7 @@ double *Storage::device_overwrite() {
   write_stamp_++;
   settle_upload();
   ensure_device_buffer();
+  note_step();
   zero_ = false;
   dev_valid_ = true;
   host_valid_ = false;
@@ -262,6 +279,7 @@ double *Storage::device_accumulate(bool *store) {
   }
   if (zero_) {
     ensure_device_buffer();
+    note_step();
     *store = true;
     zero_ = false;
     dev_valid_ = true;
@@ -272,6 +290,7 @@ double *Storage::device_accumulate(bool *store) {
   if (!dev_valid_) {
     sync_device_from_host();
   }
+  note_step();
   host_valid_ = false;
   return dev_;
 }
@@ -298,6 +317,7 @@ void Storage::fill(double value) {
   write_stamp_++;
   settle_upload();
   ensure_device_buffer();
+  note_step();
   check(mg_fill(dev_, value, size_), "fill");
   zero_ = false;
   dev_valid_ = true;

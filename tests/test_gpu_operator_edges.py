@@ -99,3 +99,51 @@ def test_codes_between_two_steps(abi, n):
     abi.mg_q8_pack(dx.ptr, packed.codes.ptr, packed.scales.ptr, m, n)
     codes, scales = packed.read()
     assert np.array_equal(codes, want_codes) and np.array_equal(scales, want_scales)
+
+
+def recorded(api, body):
+    """`body` as a recorded step, which is closed whatever happens in it."""
+    rec = api.RecordedStep()
+    rec.begin()
+    try:
+        out = body()
+    finally:
+        rec.end()
+    return rec, out
+
+
+def test_a_buffer_that_a_recorded_step_uses_is_not_given_up(api, abi):
+    rng = np.random.default_rng(7)
+    m, n = 20, 70
+    first, second = rng.standard_normal((2, m, n))
+    x, w = api.Tensor([m, n], first), api.Tensor([n, 8], rng.standard_normal((n, 8)))
+    x.set_requires_grad(False)
+    warm = x.matmul(w).sum()
+    del warm
+    rec, out = recorded(api, lambda: x.matmul(w).sum())
+    for t in (x, w):
+        with pytest.raises(RuntimeError, match="a recorded step uses"):
+            t.keep_8bit()
+        assert not t.kept_8bit()
+    x.copy_from_host(second)
+    rec.replay()
+    want = float((second @ w.data().reshape(n, 8)).sum())
+    assert abs(out.data()[0] - want) <= 1e-11 * np.abs(second).sum()
+    # a tensor that no step uses may still be kept
+    other = api.Tensor([m, n], first)
+    other.keep_8bit()
+    assert other.kept_8bit()
+    # the fp64 form of a kept tensor, once a step has read it, stays where it is
+    other.add(1.0)
+    rec2, out2 = recorded(api, lambda: other.add(1.0))
+    other.keep_8bit()
+    filler = [api.Tensor([m, n], np.full((m, n), 9.0)) for _ in range(4)]
+    rec2.replay()
+    assert np.array_equal(out2.data(), other.data() + 1.0) and len(filler) == 4
+    # ... and is given up once no step is left that may use it
+    assert abi.mg_graph_count() >= 2
+    del rec, rec2, out, out2
+    if abi.mg_graph_count() == 0:  # (other tests may have left one)
+        x.keep_8bit()
+        assert x.kept_8bit()
+    abi.mg_check_kernel_status()
