@@ -107,7 +107,8 @@ public:
   // any write to the tensor ends the 8-bit form.  Refused (std::logic_error) for tensors
   // whose values share a buffer (parameters after SGD::enable_allreduce, load_mnist
   // samples), for tensors that a recorded step has used (its replays use the buffer where
-  // it was; until no recorded step is left), and, while a step is recorded, for tensors made before the recording.
+  // it was; until no recorded step is left), and, while a step is recorded, for tensors made before the recording.  A step
+  // that is recorded cannot use a tensor that was kept in 8 bits before it.
   void keep_8bit();
   bool kept_8bit() const;
   // Read-only host views.  Unlike the mutable data()/grad() of the reference

@@ -75,7 +75,9 @@ public:
   // of them again (the codes stay), any write drops the codes.
   void pack8(size_t rows, size_t cols);
   bool packed() const { return codes_ != nullptr; }
-  const signed char *codes() const { return codes_; }
+  // The codes, for a kernel.  Refused while a step is recorded unless that step made
+  // them: a later write gives them up, and replays would go on reading them.
+  const signed char *codes();
   const double *scales() const { return scales_; }
   // True when the device buffer holds the current values (not logical zeros,
   // not superseded by a lent host view).

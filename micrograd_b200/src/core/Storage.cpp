@@ -56,6 +56,13 @@ void Storage::note_step() {
   }
 }
 
+const signed char *Storage::codes() {
+  if (!codes_recorded_ && mg_graph_recording()) {
+    throw std::logic_error("a tensor kept in 8 bits before a recording is used on the other side of it");
+  }
+  return codes_;
+}
+
 void Storage::pack8(size_t rows, size_t cols) {
   if (zero_ || size_ == 0) {
     return;  // nothing to keep
@@ -129,7 +136,11 @@ void Storage::download(double *values, size_t first, size_t n) {
     check(mg_download(values, dev_ + first, n), "download");
     return;
   }
-  // From the codes, whatever side of a recording they were made on.
+  // From the codes, whatever side of a recording they were made on (none of this may
+  // become part of a step).
+  if (mg_graph_recording()) {
+    throw std::logic_error("a tensor kept in 8 bits is read by the host while a step is recorded");
+  }
   double *fp64 = nullptr;
   check(mg_alloc(size_, &fp64), "device allocation");
   int rc = mg_q8_unpack(codes_, scales_, fp64, code_rows_, code_cols_);

@@ -147,3 +147,27 @@ def test_a_buffer_that_a_recorded_step_uses_is_not_given_up(api, abi):
         x.keep_8bit()
         assert x.kept_8bit()
     abi.mg_check_kernel_status()
+
+
+@pytest.mark.parametrize("use", ["product", "mask"])
+def test_codes_made_before_a_recording_are_not_read_by_it(api, abi, use):
+    """A write outside the step gives such codes up, and replays would go on reading them."""
+    rng = np.random.default_rng(8)
+    m, n = 12, 70
+    t = api.Tensor([m, n], rng.standard_normal((m, n)))
+    w = api.Tensor([n, 5], rng.standard_normal((n, 5)))
+    loss = (t.matmul(w) if use == "product" else t.relu()).sum()
+    if use == "product":
+        t.set_requires_grad(False)
+    t.keep_8bit()
+    values = []
+
+    def body():
+        with pytest.raises(RuntimeError, match="other side"):
+            loss.backward()
+        with pytest.raises(RuntimeError):  # (and the host does not read them into the step)
+            values.append(t.data())
+
+    rec, _ = recorded(api, body)
+    assert t.kept_8bit() and not values and np.all(np.isfinite(t.data()))
+    abi.mg_check_kernel_status()
