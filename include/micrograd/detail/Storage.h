@@ -96,6 +96,7 @@ private:
   void sync_device_from_host();
   void sync_host_from_device();
   void drop_codes();     // the contents are about to be replaced
+  void refuse_host_write() const;
   void note_step();      // a pointer to dev_ is handed out
   void expand();         // dev_ from the codes
   void download(double *values, size_t first, size_t n);  // current device contents, from either form

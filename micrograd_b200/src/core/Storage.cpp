@@ -40,12 +40,36 @@ Storage::~Storage() {
   drop_codes();
 }
 
+// Codes that were dropped while a step was being recorded which did not make them: a free
+// would become part of the step.  They go with the next ones dropped outside.
+static std::vector<void *> g_parked_codes;
+
 void Storage::drop_codes() {
-  if (codes_) {
+  if (!codes_) {
+    return;
+  }
+  const bool recording = mg_graph_recording() != 0;
+  if (!recording) {
+    for (void *buf : g_parked_codes) {
+      mg_free(static_cast<double *>(buf));
+    }
+    g_parked_codes.clear();
+  }
+  if (recording && !codes_recorded_) {
+    g_parked_codes.push_back(codes_);
+    g_parked_codes.push_back(scales_);
+  } else {
     mg_free_i8(codes_);
     mg_free(scales_);
-    codes_ = nullptr;
-    scales_ = nullptr;
+  }
+  codes_ = nullptr;
+  scales_ = nullptr;
+}
+
+// A host write that a recording would refuse must not have given up the values before.
+void Storage::refuse_host_write() const {
+  if (codes_ && mg_graph_recording()) {
+    throw std::logic_error("a tensor kept in 8 bits is written by the host while a step is recorded");
   }
 }
 
@@ -336,6 +360,7 @@ void Storage::fill(double value) {
 }
 
 std::vector<double> &Storage::host_mutable() {
+  refuse_host_write();
   host_const();  // (before the stamp moves: a pending scalar mirror is still current here)
   if (zero_) {
     zero_ = false;  // the zeros just written to host_ are now the contents
@@ -380,6 +405,7 @@ double Storage::peek(size_t index) {
 }
 
 void Storage::upload_in_place(const double *values) {
+  refuse_host_write();
   drop_codes();
   write_stamp_++;
   settle_upload();
@@ -391,6 +417,7 @@ void Storage::upload_in_place(const double *values) {
 }
 
 void Storage::prefetch_in_place(const double *values) {
+  refuse_host_write();
   drop_codes();
   write_stamp_++;
   settle_upload();  // an earlier prefetch into the same buffer is ordered first

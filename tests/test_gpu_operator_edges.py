@@ -171,3 +171,34 @@ def test_codes_made_before_a_recording_are_not_read_by_it(api, abi, use):
     rec, _ = recorded(api, body)
     assert t.kept_8bit() and not values and np.all(np.isfinite(t.data()))
     abi.mg_check_kernel_status()
+
+
+def test_a_write_during_a_recording_loses_no_kept_values(api, abi):
+    rng = np.random.default_rng(12)
+    m, n = 9, 130
+    x = rng.standard_normal((m, n))
+    t, p = api.Tensor([m, n], x), api.Tensor([m, n], x)
+    opt = api.SGD([p], 0.5)
+    p.sum().backward()
+    opt.step()  # (once before the recording)
+    for v in (t, p):
+        v.keep_8bit()
+    kept, before = t.data().copy(), p.data().copy()
+    p.add(0.0)  # (its fp64 form exists, for the step below)
+
+    def body():
+        for write in (lambda: t.copy_from_host(x), lambda: t.set_at([0, 0], 3.0)):
+            with pytest.raises(RuntimeError):
+                write()
+        opt.step()
+
+    rec, _ = recorded(api, body)
+    assert t.kept_8bit() and np.array_equal(t.data(), kept)
+    assert not p.kept_8bit()
+    for _ in range(2):
+        rec.replay()
+        before = before - 0.5  # (rounded step by step, as the kernel does)
+        assert np.array_equal(p.data(), before)
+    t.copy_from_host(x)  # (gives up the parked codes, too)
+    assert not t.kept_8bit() and np.array_equal(t.data(), x.reshape(-1))
+    abi.mg_check_kernel_status()
