@@ -277,18 +277,27 @@ static GemmPlan choose_plan(int M, int N, int K, int sms, int shape) {
 // ---------------------------------------------------------------------------
 // Segment tables of split contractions.  A table depends only on the tile grid,
 // the k-tile count and the span count, so it is built once per shape and kept
-// on the device until shutdown.
+// on the device: the 256 latest ones, and those that the kernels of a recorded step
+// read (their addresses are part of the step) as long as any step exists.
 // ---------------------------------------------------------------------------
 static std::vector<SegTable> g_seg_tables;
+constexpr size_t kMostTables = 256;
 
-void gemm_release_tables() {
+static void release_tables(bool recorded_too) {
+  std::vector<SegTable> kept;
   for (auto &t : g_seg_tables) {
+    if (t.recorded && !recorded_too) {
+      kept.push_back(t);
+      continue;
+    }
     cudaFree(t.dev_items);
     cudaFree(t.dev_tickets);
     cudaFree(t.dev_tiles);
   }
-  g_seg_tables.clear();
+  g_seg_tables.swap(kept);
 }
+
+void gemm_release_tables() { release_tables(true); }
 
 // After a kernel fault (a bounded wait gave up) a split tile may be left with a
 // partly counted ticket; clear them all so later launches start clean.
@@ -351,9 +360,10 @@ static void build_segments(int tiles_m, int tiles_n, int KT, int bm, int bn, int
 
 int seg_table_for(int tiles_m, int tiles_n, int KT, int bm, int bn, int spans,
                          const SegTable **out) {
-  for (const auto &t : g_seg_tables) {
+  for (auto &t : g_seg_tables) {
     if (t.tiles_m == tiles_m && t.tiles_n == tiles_n && t.KT == KT && t.bm == bm && t.bn == bn &&
         t.spans == spans) {
+      t.recorded = t.recorded || ctx().capturing;
       *out = &t;
       return MG_OK;
     }
@@ -365,7 +375,9 @@ int seg_table_for(int tiles_m, int tiles_n, int KT, int bm, int bn, int spans,
   // A job with ever-changing shapes (e.g. a varying batch) would grow the cache
   // without bound: start over beyond 256 tables (cudaFree waits for the kernels
   // that still read them).
-  if (g_seg_tables.size() >= 256) gemm_release_tables();
+  size_t loose = 0;
+  for (const auto &t : g_seg_tables) loose += t.recorded ? 0 : 1;
+  if (loose >= kMostTables) release_tables(mg_graph_count() == 0);
   std::vector<SegItem> segs;
   std::vector<int2> tile_info;
   int slots = 0, min_nkt = KT;

@@ -731,6 +731,7 @@ struct SegTable {
   SegItem *dev_items;  // [items], longest first
   unsigned int *dev_tickets;  // [tiles]: arrival counters of the in-kernel fold, zero between launches
   int2 *dev_tiles;            // [tiles]: first slot and segment count of a split tile, (0, 0) of a whole one
+  bool recorded;              // a recorded step reads it
 };
 
 int choose_spans(int tiles, int KT, int sms);

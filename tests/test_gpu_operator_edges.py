@@ -1,4 +1,6 @@
 """GPU: the operators for larger models at the edges of what they accept."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -202,4 +204,41 @@ def test_a_write_during_a_recording_loses_no_kept_values(api, abi):
         assert np.array_equal(p.data(), before)
     t.copy_from_host(x)  # (gives up the parked codes, too)
     assert not t.kept_8bit() and np.array_equal(t.data(), x.reshape(-1))
+    abi.mg_check_kernel_status()
+
+
+def test_a_recorded_product_outlives_the_table_cache(abi):
+    """Products of 600 other shapes, more than the cache of split contractions holds, run
+    between a recording and its replays."""
+    rng = np.random.default_rng(11)
+    m, n, k = 4100, 64, 48  # weight gradient: the contraction over m is split
+    a, g = rng.standard_normal((m, k)), rng.standard_normal((m, n))
+    da, dg, out = abi.array(a), abi.array(g), abi.empty(k * n)
+    abi.mg_gemm_tn(da.ptr, dg.ptr, out.ptr, m, n, k, 0)
+    want = out.numpy()
+    codes, scales = encode(a)
+    packed, out8 = Packed(abi, m, k, codes, scales), abi.empty(k * n)
+    abi.mg_gemm_tn_q8(packed.codes.ptr, packed.scales.ptr, dg.ptr, out8.ptr, m, n, k, 0)
+    want8 = out8.numpy()
+    step = C.c_int()
+    abi.mg_graph_begin()
+    abi.mg_gemm_tn(da.ptr, dg.ptr, out.ptr, m, n, k, 0)
+    abi.mg_gemm_tn_q8(packed.codes.ptr, packed.scales.ptr, dg.ptr, out8.ptr, m, n, k, 0)
+    abi.mg_graph_end(C.byref(step))
+    big, small = abi.zeros(16 * 1300 * 16), abi.empty(256)
+    for i in range(600):
+        abi.mg_gemm_tn(big.ptr, big.ptr, small.ptr, 16 * (600 + i), 16, 16, 0)
+    for _ in range(3):
+        abi.mg_fill(out.ptr, 7.0, k * n)
+        abi.mg_fill(out8.ptr, 7.0, k * n)
+        abi.mg_graph_launch(step.value)
+        assert np.array_equal(out.numpy(), want) and np.array_equal(out8.numpy(), want8)
+    # ... and the same products, one launch at a time, are still what they were
+    abi.mg_gemm_tn(da.ptr, dg.ptr, out.ptr, m, n, k, 0)
+    assert np.array_equal(out.numpy(), want)
+    abi.mg_graph_destroy(step.value)
+    for i in range(600):  # (without a recorded step the tables go again)
+        abi.mg_gemm_tn(big.ptr, big.ptr, small.ptr, 16 * (600 + i), 16, 16, 0)
+    abi.mg_gemm_tn(da.ptr, dg.ptr, out.ptr, m, n, k, 0)
+    assert np.array_equal(out.numpy(), want)
     abi.mg_check_kernel_status()
