@@ -289,7 +289,9 @@ int mg_q8_unpack(const signed char *codes, const double *scales, double *x, size
  * MG_EPI_RELU_MASK, their A operand / mask source in 8 bits:
  *   dB[K,N] (+)= x[M,K]^T . G[M,N],  x = the values codes and scales keep (in pieces of
  *                rows, in a workspace of at most 256 MiB or 64 rows, where N > 32);
- *   dA[M,K] (+)= (G[M,N] . B[K,N]^T) * (mask_codes[M,K] > 0);
+ *   dA[M,K] (+)= (G[M,N] . B[K,N]^T) * (mask_codes[M,K] > 0)  (where N > 16 is odd, or G
+ *                or B off a 16-byte boundary: in pieces of rows, in a workspace of at most
+ *                256 MiB or 128 rows, and one of B's size);
  * and the ReLU mask alone: gx[n] += g[n] * (codes[n] > 0). */
 int mg_gemm_tn_q8(const signed char *codes, const double *scales, const double *G, double *dB,
                   size_t M, size_t N, size_t K, int accumulate);

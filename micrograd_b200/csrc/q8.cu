@@ -624,7 +624,8 @@ static int unpack_rows(const signed char *codes, const double *scales, double *x
   return MG_OK;
 }
 
-// fp64 values held at a time for a weight gradient.
+// fp64 values held at a time for a weight gradient, and for the rows of an input gradient
+// that have to be copied.
 constexpr size_t kQ8UnpackBytes = (size_t)256 << 20;
 
 static int check_q8(const char *name, size_t M, size_t N) {
@@ -732,16 +733,26 @@ int mg_gemm_nt_q8(const double *G, const double *B, double *dA, size_t M, size_t
   GemmExt e{{G, B, dA, M, K, N, true, true, accumulate, MG_EPI_NONE, nullptr}};
   e.mask8 = mask_codes;
   if (N % 2 == 0 && !off_16_bytes(G) && !off_16_bytes(B)) return run_gemm_ext(e);
+  // Odd rows, or rows off a 16-byte boundary: B is copied once into rows the tensor kernel
+  // can take, G in pieces of as many rows as kQ8UnpackBytes hold.
   const size_t pitch = pitch16(N);
+  size_t rows = kQ8UnpackBytes / 8 / pitch / 128 * 128;
+  if (rows < 128) rows = 128;
+  if (rows > M) rows = M;
   double *room = nullptr;
-  int rc = mg_alloc((M + K) * pitch, &room);
+  int rc = mg_alloc((rows + K) * pitch, &room);
   if (rc != MG_OK) return rc;
-  rc = copy_rows(G, M, N, N, room, pitch);
-  if (rc == MG_OK) rc = copy_rows(B, K, N, N, room + M * pitch, pitch);
+  rc = copy_rows(B, K, N, N, room + rows * pitch, pitch);
   e.d.A = room;
-  e.d.B = room + M * pitch;
+  e.d.B = room + rows * pitch;
   e.lda = e.ldb = pitch;
-  if (rc == MG_OK) rc = run_gemm_ext(e);
+  for (size_t m = 0; m < M && rc == MG_OK; m += rows) {
+    e.d.M = M - m < rows ? M - m : rows;
+    e.d.D = dA + m * K;
+    e.mask8 = mask_codes + m * K;
+    rc = copy_rows(G + m * N, e.d.M, N, N, room, pitch);
+    if (rc == MG_OK) rc = run_gemm_ext(e);
+  }
   const int freed = mg_free(room);
   return rc != MG_OK ? rc : freed;
 }

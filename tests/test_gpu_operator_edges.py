@@ -1,5 +1,8 @@
 """GPU: the operators for larger models at the edges of what they accept."""
 import ctypes as C
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -242,3 +245,44 @@ def test_a_recorded_product_outlives_the_table_cache(abi):
     abi.mg_gemm_tn(da.ptr, dg.ptr, out.ptr, m, n, k, 0)
     assert np.array_equal(out.numpy(), want)
     abi.mg_check_kernel_status()
+
+
+def memory_growth(setup, small, call):
+    """Bytes by which the device's used memory grows in `call`, in a process of its own;
+    `small` has run all of its kernels before."""
+    code = ("import ctypes as C, sys\nsys.path.insert(0, %r)\nimport micrograd_b200\nabi = micrograd_b200.load_abi()\nabi.mg_init(-1)\n"
+            "def used():\n    f, t = C.c_size_t(), C.c_size_t()\n    abi.mg_sync()\n    abi.mg_mem_info(C.byref(f), C.byref(t))\n"
+            "    return t.value - f.value\n%s\n%s\nbefore = used()\n%s\nprint(used() - before)\n"
+            % (os.path.dirname(os.path.dirname(os.path.abspath(__file__))), setup, small, call))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+    return int(r.stdout.split()[-1])
+
+
+def test_workspace_of_the_masked_input_gradient(abi):
+    """3 million rows of 17 columns (copied to 32 in the workspace, 768 MB as a whole) are
+    taken in pieces of at most 256 MiB; the pool may add 64."""
+    setup = ("m, n, k = 3000001, 17, 2\ng, w, dx, codes = abi.zeros(m * n), abi.zeros(n * k), abi.empty(m * k), abi.zeros(m * k // 8 + 1)")
+    call = "abi.mg_gemm_nt_q8(g.ptr, w.ptr, dx.ptr, %s, n, k, 0, codes.ptr)"
+    assert memory_growth(setup, call % 1000, call % "m") <= (256 + 64) << 20
+
+
+def test_masked_input_gradient_in_pieces(abi):
+    """The rows at the ends of the pieces (a piece holds 256 MiB / 8 / 32 = 1 048 576 rows)
+    and the last one, with and without accumulation."""
+    m, n, k = 2100003, 17, 3
+    piece = 1 << 20
+    rows = np.array([0, 1, piece - 1, piece, piece + 1, 2 * piece - 1, 2 * piece, m - 1])
+    rng = np.random.default_rng(9)
+    g, w = rng.standard_normal((m, n)), rng.standard_normal((k, n))
+    codes, old = rng.integers(-2, 3, (m, k)).astype(np.int8), rng.standard_normal((m, k))
+    packed, dg, dw = Packed(abi, m, k, codes, np.zeros(1)), abi.array(g), abi.array(w)
+    for acc in (0, 1):
+        out = abi.array(old)
+        abi.mg_gemm_nt_q8(dg.ptr, dw.ptr, out.ptr, m, n, k, acc, packed.codes.ptr)
+        got = out.numpy((m, k))
+        ref = (g @ w.T) * (codes > 0) + acc * old
+        bound = (2 * n + 6) * U * (np.abs(g) @ np.abs(w).T + np.abs(old))  # (numpy's own errors too)
+        assert np.all(np.abs(got - ref) <= bound)
+        exact = (g[rows].astype(LD) @ w.T.astype(LD)) * (codes[rows] > 0) + acc * old[rows]
+        assert np.all(np.abs(got[rows] - exact) <= bound[rows])
