@@ -288,7 +288,8 @@ int mg_q8_unpack(const signed char *codes, const double *scales, double *x, size
 /* The backward pass on the 8-bit form.  mg_gemm_tn and mg_gemm_nt with
  * MG_EPI_RELU_MASK, their A operand / mask source in 8 bits:
  *   dB[K,N] (+)= x[M,K]^T . G[M,N],  x = the values codes and scales keep (in pieces of
- *                rows, in a workspace of at most 256 MiB or 64 rows, where N > 32);
+ *                rows, in a workspace of at most 256 MiB or 64 rows, where N > 32; of twice
+ *                that where rows of G are odd, or off a 16-byte boundary, and are copied too);
  *   dA[M,K] (+)= (G[M,N] . B[K,N]^T) * (mask_codes[M,K] > 0)  (where N > 16 is odd, or G
  *                or B off a 16-byte boundary: in pieces of rows, in a workspace of at most
  *                256 MiB or 128 rows, and one of B's size);

@@ -699,7 +699,7 @@ int mg_gemm_tn_q8(const signed char *codes, const double *scales, const double *
   // hold up the tensor instructions; 4.32 ms against 4.05 at 65 536 x 1024 x 1024.)
   const size_t pitch = pitch16(K), pitch_g = pitch16(N);
   const bool copy_g = N % 2 != 0 || off_16_bytes(G);
-  size_t rows = kQ8UnpackBytes / 8 / pitch / 64 * 64;
+  size_t rows = kQ8UnpackBytes / 8 / (copy_g && pitch_g > pitch ? pitch_g : pitch) / 64 * 64;
   if (rows < 64) rows = 64;
   if (rows > M) rows = M;
   double *room = nullptr;

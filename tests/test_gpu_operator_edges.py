@@ -9,7 +9,7 @@ import pytest
 
 from micrograd_b200 import cabi as K
 from test_gpu_group_norm import call_fwd, near
-from test_gpu_q8 import Packed, encode
+from test_gpu_q8 import Packed, activation, encode
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -53
@@ -286,3 +286,26 @@ def test_masked_input_gradient_in_pieces(abi):
         assert np.all(np.abs(got - ref) <= bound)
         exact = (g[rows].astype(LD) @ w.T.astype(LD)) * (codes[rows] > 0) + acc * old[rows]
         assert np.all(np.abs(got[rows] - exact) <= bound[rows])
+
+
+def test_workspace_of_the_weight_gradient(abi):
+    """100 000 rows of 16 kept and 1001 other columns (copied to 1008, 806 MB as a whole): at
+    most 256 MiB for each; the pool may add 64."""
+    setup = "m, n, k = 100000, 1001, 16\ng, codes, scales, dw = abi.zeros(m * n), abi.zeros(m * k // 8 + 1), abi.zeros(m), abi.empty(n * k)"
+    call = "abi.mg_gemm_tn_q8(codes.ptr, scales.ptr, g.ptr, dw.ptr, %s, n, k, 0)"
+    assert memory_growth(setup, call % 1000, call % "m") <= (512 + 64) << 20
+
+
+def test_weight_gradient_in_pieces(abi):
+    """Rows of 1008 doubles in the workspace: pieces of 33 280 rows."""
+    m, n, k = 70001, 1001, 10
+    rng, x = activation(m, k, 14)
+    codes, scales = encode(x)
+    g, old = rng.standard_normal((m, n)), rng.standard_normal((k, n))
+    values = codes * np.repeat(scales, 64, axis=1)[:, :k]
+    packed, dg = Packed(abi, m, k, codes, scales), abi.array(g)
+    bound = (2 * m + 8) * U * (np.abs(values).T @ np.abs(g) + np.abs(old))  # (numpy's own errors too)
+    for acc in (0, 1):
+        out = abi.array(old)
+        abi.mg_gemm_tn_q8(packed.codes.ptr, packed.scales.ptr, dg.ptr, out.ptr, m, n, k, acc)
+        assert np.all(np.abs(out.numpy((k, n)) - (values.T @ g + old * acc)) <= bound)
