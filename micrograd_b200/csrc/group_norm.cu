@@ -192,65 +192,63 @@ gn_apply_kernel(const double *__restrict__ x, const double *__restrict__ gamma,
   }
 }
 
-// Backward, step 1: sums of gz and gz unit over one piece of a sample's positions,
-// per channel: parts[n][piece][2][C].
+// Backward, step 1: sums of u and u unit over one piece of one group; with one piece they
+// are its m1 and m2.
 template <int ACT>
 __global__ void __launch_bounds__(kGnThreads)
-gn_bwd_sums_kernel(const double *__restrict__ x, const double *__restrict__ gamma,
-                   const double *__restrict__ beta, const double *__restrict__ mean,
-                   const double *__restrict__ rstd, const double *__restrict__ gy, NormShape s,
-                   unsigned pieces, size_t piece, double *__restrict__ parts) {
-  __shared__ double sums[2][8][33];
-  const int tx = threadIdx.x, ty = threadIdx.y, c = blockIdx.x * 32 + tx;
-  for (size_t unit_id = blockIdx.y; unit_id < s.N * pieces; unit_id += gridDim.y) {
-    const size_t n = unit_id / pieces, k = unit_id - n * pieces;
-    const size_t end = (k + 1) * piece < s.P ? (k + 1) * piece : s.P;
-    double sb = 0.0, sg = 0.0;
-    if (c < s.C) {
-      const size_t ng = n * s.G + c / s.D;
-      const double ga = gamma ? gamma[c] : 1.0, be = beta ? beta[c] : 0.0, mu = mean[ng], rs = rstd[ng];
-      for (size_t p = k * piece + ty; p < end; p += 8) {
-        const size_t at = (n * s.P + p) * s.C + c;
-        const double unit = (x[at] - mu) * rs, gz = act_bwd<ACT>(unit * ga + be, gy[at]);
-        sb += gz;
-        sg += gz * unit;
-      }
+gn_bwd_groups_kernel(const double *__restrict__ x, const double *__restrict__ gamma,
+                     const double *__restrict__ beta, const double *__restrict__ mean,
+                     const double *__restrict__ rstd, const double *__restrict__ gy, NormShape s,
+                     size_t piece, double *__restrict__ parts, double *__restrict__ m12) {
+  __shared__ double smem32[32];
+  const size_t ng = blockIdx.x, n = ng / s.G;
+  const int c0 = (int)(ng - n * s.G) * s.D;
+  const size_t E = s.P * (size_t)s.D;
+  const size_t begin = blockIdx.y * piece, end = begin + piece < E ? begin + piece : E;
+  const double mu = mean[ng], rs = rstd[ng];
+  // Position and channel of the values e, e + kGnThreads, ... without a division for each.
+  size_t e = begin + threadIdx.x, at = e / s.D;
+  int d = (int)(e - at * s.D);
+  at = (n * s.P + at) * s.C + c0;
+  const int rows = kGnThreads / s.D, columns = kGnThreads - rows * s.D;
+  double s1 = 0.0, s2 = 0.0;
+  for (; e < end; e += kGnThreads) {
+    const double ga = gamma ? __ldg(gamma + c0 + d) : 1.0, be = beta ? __ldg(beta + c0 + d) : 0.0;
+    const double unit = (x[at + d] - mu) * rs, u = act_bwd<ACT>(fma(unit, ga, be), gy[at + d]) * ga;
+    s1 += u;
+    s2 = fma(u, unit, s2);
+    at += (size_t)rows * s.C;
+    d += columns;
+    if (d >= s.D) {
+      d -= s.D;
+      at += s.C;
     }
-    sums[0][ty][tx] = sb;
-    sums[1][ty][tx] = sg;
-    __syncthreads();
-    if (ty < 2 && c < s.C) {
-      double t = 0.0;
-      for (int j = 0; j < 8; j++) t += sums[ty][j][tx];
-      parts[(unit_id * 2 + ty) * s.C + c] = t;
-    }
-    __syncthreads();
   }
+  s1 = cta_sum(s1, smem32);
+  s2 = cta_sum(s2, smem32);
+  if (threadIdx.x != 0) return;
+  double *out = gridDim.y == 1 ? m12 + 2 * ng : parts + 2 * (ng * gridDim.y + blockIdx.y);
+  out[0] = gridDim.y == 1 ? s1 / (double)E : s1;
+  out[1] = gridDim.y == 1 ? s2 / (double)E : s2;
 }
 
-// Step 2: m1 and m2 of every group, a warp per group.
+// Step 2: the pieces of a group joined, a warp per group.
 __global__ void __launch_bounds__(kGnThreads)
-gn_bwd_groups_kernel(const double *__restrict__ parts, const double *__restrict__ gamma, NormShape s,
-                     unsigned pieces, double *__restrict__ m12) {
+gn_bwd_groups_join_kernel(const double *__restrict__ parts, size_t groups, unsigned pieces, double E,
+                          double *__restrict__ m12) {
   const int lane = threadIdx.x & 31;
   const size_t ng = ((size_t)blockIdx.x * kGnThreads + threadIdx.x) >> 5;
-  if (ng >= s.N * s.G) return;
-  const size_t n = ng / s.G;
-  const int c0 = (int)(ng - n * s.G) * s.D;
-  double m1 = 0.0, m2 = 0.0;
-  for (size_t i = lane; i < (size_t)pieces * s.D; i += 32) {
-    const size_t k = i / s.D;
-    const int c = c0 + (int)(i - k * s.D);
-    const double ga = gamma ? gamma[c] : 1.0;
-    m1 += ga * parts[((n * pieces + k) * 2) * s.C + c];
-    m2 += ga * parts[((n * pieces + k) * 2 + 1) * s.C + c];
+  if (ng >= groups) return;
+  double s1 = 0.0, s2 = 0.0;
+  for (unsigned k = lane; k < pieces; k += 32) {
+    s1 += parts[2 * (ng * pieces + k)];
+    s2 += parts[2 * (ng * pieces + k) + 1];
   }
-  m1 = shfl_sum(m1);
-  m2 = shfl_sum(m2);
+  s1 = shfl_sum(s1);
+  s2 = shfl_sum(s2);
   if (lane == 0) {
-    const double E = (double)s.P * s.D;
-    m12[2 * ng] = m1 / E;
-    m12[2 * ng + 1] = m2 / E;
+    m12[2 * ng] = s1 / E;
+    m12[2 * ng + 1] = s2 / E;
   }
 }
 
@@ -314,24 +312,50 @@ static int sum_params(double *parts, size_t rows, int C, double *ggamma, double 
   return MG_OK;
 }
 
-// Step 3: the input's gradient.
+// Step 3: the input's gradient (gx may be null), and the sums of gz and gz unit over the
+// rows (n, p) that a CTA walks, per channel: parts[blockIdx.y][2][C] (or null).  The sums
+// stay in the threads until the end, so that they take no more memory than there are CTAs.
 template <int ACT>
 __global__ void __launch_bounds__(kGnThreads)
 gn_bwd_apply_kernel(const double *__restrict__ x, const double *__restrict__ gamma,
                     const double *__restrict__ beta, const double *__restrict__ mean,
                     const double *__restrict__ rstd, const double *__restrict__ gy,
-                    const double *__restrict__ m12, double *gx, bool accumulate, NormShape s) {
-  const int c = blockIdx.x * 32 + threadIdx.x;
-  if (c >= s.C) return;
-  const int g = c / s.D;
-  const double ga = gamma ? gamma[c] : 1.0, be = beta ? beta[c] : 0.0;
-  const size_t rows = s.N * s.P;
-  for (size_t r = (size_t)blockIdx.y * blockDim.y + threadIdx.y; r < rows; r += (size_t)gridDim.y * blockDim.y) {
-    const size_t ng = r / s.P * s.G + g, at = r * s.C + c;
-    const double rs = __ldg(rstd + ng), unit = (x[at] - __ldg(mean + ng)) * rs;
-    const double u = act_bwd<ACT>(unit * ga + be, gy[at]) * ga;
-    const double v = rs * (u - __ldg(m12 + 2 * ng) - unit * __ldg(m12 + 2 * ng + 1));
-    gx[at] = accumulate ? gx[at] + v : v;
+                    const double *__restrict__ m12, double *gx, bool accumulate, NormShape s,
+                    double *__restrict__ parts) {
+  __shared__ double sums[2][8][33];
+  const int tx = threadIdx.x, ty = threadIdx.y, c = blockIdx.x * 32 + tx;
+  double sb = 0.0, sg = 0.0;
+  if (c < s.C) {
+    const int g = c / s.D;
+    const double ga = gamma ? gamma[c] : 1.0, be = beta ? beta[c] : 0.0;
+    const size_t rows = s.N * s.P, step = (size_t)gridDim.y * 8, step_n = step / s.P, step_p = step - step_n * s.P;
+    size_t r = (size_t)blockIdx.y * 8 + ty, n = r / s.P, p = r - n * s.P;
+    for (; r < rows; r += step) {
+      const size_t ng = n * s.G + g, at = r * s.C + c;
+      const double rs = __ldg(rstd + ng), unit = (x[at] - __ldg(mean + ng)) * rs;
+      const double gz = act_bwd<ACT>(fma(unit, ga, be), gy[at]);
+      sb += gz;
+      sg = fma(gz, unit, sg);
+      if (gx) {
+        const double v = rs * (gz * ga - __ldg(m12 + 2 * ng) - unit * __ldg(m12 + 2 * ng + 1));
+        gx[at] = accumulate ? gx[at] + v : v;
+      }
+      n += step_n;
+      p += step_p;
+      if (p >= s.P) {
+        p -= s.P;
+        n++;
+      }
+    }
+  }
+  if (!parts) return;
+  sums[0][ty][tx] = sb;
+  sums[1][ty][tx] = sg;
+  __syncthreads();
+  if (ty < 2 && c < s.C) {
+    double t = 0.0;
+    for (int j = 0; j < 8; j++) t += sums[ty][j][tx];
+    parts[((size_t)blockIdx.y * 2 + ty) * s.C + c] = t;
   }
 }
 
@@ -405,34 +429,40 @@ static int general_bwd(const double *x, const double *gamma, const double *beta,
                        const double *rstd, const double *gy, double *gx, double *ggamma, double *gbeta,
                        const NormShape &s, int act, int flags) {
   Context &c = ctx();
-  // A piece of 256 positions costs 16 C bytes of sums for 4096 C bytes of data.
-  const size_t piece = 256, pieces = (s.P + piece - 1) / piece, rows = s.N * pieces;
+  const size_t E = s.P * (size_t)s.D, groups = s.N * s.G;
+  size_t pieces = (E + kGnPiece - 1) / kGnPiece;
+  if (pieces > 65535) pieces = 65535;
+  const size_t piece = (E + pieces - 1) / pieces;
+  pieces = (E + piece - 1) / piece;
+  const dim3 grid = rows_grid(s, (s.N * s.P + 7) / 8);
+  const size_t n_rows = (grid.y + param_layers(grid.y)) * 2 * (size_t)s.C;
   double *parts = nullptr;
-  const size_t room = (rows + param_layers(rows)) * 2 * s.C;
-  int rc = scratch(room + 2 * s.N * s.G, &parts);
+  int rc = scratch(n_rows + 2 * groups * (pieces > 1 ? pieces + 1 : 1), &parts);
   if (rc != MG_OK) return rc;
-  double *m12 = parts + room;
-  rc = by_activation(act, [&](auto a) {
-    gn_bwd_sums_kernel<decltype(a)::value><<<rows_grid(s, rows), dim3(32, 8), 0, c.stream>>>(
-        x, gamma, beta, mean, rstd, gy, s, (unsigned)pieces, piece, parts);
-    MG_LAUNCH_CHECK("group_norm backward sums");
-    return MG_OK;
-  });
-  if (rc != MG_OK) return rc;
-  if (ggamma || gbeta) {
-    rc = sum_params(parts, rows, s.C, ggamma, gbeta, flags);
+  double *m12 = parts + n_rows, *piece_sums = m12 + 2 * groups;
+  if (gx) {
+    rc = by_activation(act, [&](auto a) {
+      gn_bwd_groups_kernel<decltype(a)::value><<<dim3((unsigned)groups, (unsigned)pieces), kGnThreads, 0, c.stream>>>(
+          x, gamma, beta, mean, rstd, gy, s, piece, piece_sums, m12);
+      MG_LAUNCH_CHECK("group_norm backward groups");
+      return MG_OK;
+    });
     if (rc != MG_OK) return rc;
+    if (pieces > 1) {
+      gn_bwd_groups_join_kernel<<<(unsigned)((groups * 32 + kGnThreads - 1) / kGnThreads), kGnThreads, 0, c.stream>>>(
+          piece_sums, groups, (unsigned)pieces, (double)E, m12);
+      MG_LAUNCH_CHECK("group_norm backward groups join");
+    }
   }
-  if (!gx) return MG_OK;
-  gn_bwd_groups_kernel<<<(unsigned)((s.N * s.G * 32 + kGnThreads - 1) / kGnThreads), kGnThreads, 0, c.stream>>>(
-      parts, gamma, s, (unsigned)pieces, m12);
-  MG_LAUNCH_CHECK("group_norm backward groups");
-  return by_activation(act, [&](auto a) {
-    gn_bwd_apply_kernel<decltype(a)::value><<<rows_grid(s, (s.N * s.P + 7) / 8), dim3(32, 8), 0, c.stream>>>(
-        x, gamma, beta, mean, rstd, gy, m12, gx, !(flags & MG_ACC_STORE_A), s);
+  const bool params = ggamma || gbeta;
+  rc = by_activation(act, [&](auto a) {
+    gn_bwd_apply_kernel<decltype(a)::value><<<grid, dim3(32, 8), 0, c.stream>>>(
+        x, gamma, beta, mean, rstd, gy, m12, gx, !(flags & MG_ACC_STORE_A), s, params ? parts : nullptr);
     MG_LAUNCH_CHECK("group_norm backward apply");
     return MG_OK;
   });
+  if (rc != MG_OK || !params) return rc;
+  return sum_params(parts, grid.y, s.C, ggamma, gbeta, flags);
 }
 
 // ---------------------------------------------------------------------------

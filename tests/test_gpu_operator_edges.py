@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 
 from micrograd_b200 import cabi as K
-from test_gpu_group_norm import call_fwd, near
+from test_gpu_group_norm import backward, call_fwd, near
 from test_gpu_q8 import Packed, activation, encode
 
 pytestmark = pytest.mark.gpu
@@ -309,3 +309,45 @@ def test_weight_gradient_in_pieces(abi):
         out = abi.array(old)
         abi.mg_gemm_tn_q8(packed.codes.ptr, packed.scales.ptr, dg.ptr, out.ptr, m, n, k, acc)
         assert np.all(np.abs(out.numpy((k, n)) - (values.T @ g + old * acc)) <= bound)
+
+
+def test_workspace_of_the_norm_of_wide_rows(abi):
+    """16 384 rows of 2049 channels in one group.  Channel sums of each row would take 537 MB;
+    what a call needs does not grow with the data, and the pool may add 64 MiB."""
+    setup = ("n, c = 16384, 2049\nx, gy, gx = abi.zeros(n * c), abi.zeros(n * c), abi.empty(n * c)\n"
+             "m, r, gg, gb = abi.zeros(n), abi.zeros(n), abi.empty(c), abi.empty(c)")
+    call = ("abi.mg_group_norm_bwd(x.ptr, None, None, m.ptr, r.ptr, gy.ptr, gx.ptr, gg.ptr, gb.ptr, %s, 1, c, 1, 2, 7)")
+    assert memory_growth(setup, call % 10, call % "n") <= (16 + 64) << 20
+
+
+@pytest.mark.parametrize("p", [1, 2])
+def test_norm_gradients_of_many_wide_rows(abi, p):
+    """Gradients of each row, and the channels' sums over all of them added to what was there."""
+    d = 2049
+    n = 9000
+    rng = np.random.default_rng(10)
+    x = abi.empty(n * p * d)
+    gy = abi.empty(n * p * d)
+    abi.mg_fill_uniform01(x.ptr, n * p * d, 3, 0)
+    abi.mg_fill_uniform01(gy.ptr, n * p * d, 4, 0)
+    xv, gv = x.numpy((n, p, 1, d)), gy.numpy((n, p, 1, d))
+    gamma, beta = 1 + 0.1 * rng.standard_normal(d), 0.1 * rng.standard_normal(d)
+    mean, rstd = xv.mean(axis=(1, 3)), 1 / np.sqrt(xv.var(axis=(1, 3)) + 1e-5)
+    m4, r4 = mean[:, None, :, None], rstd[:, None, :, None]
+    olds = [rng.standard_normal(v.shape) for v in (gamma, gamma)]
+    dev = [abi.array(v) for v in (gamma, beta, mean, rstd)]
+    gx, gg, gb = abi.empty(n * p * d), abi.array(olds[0]), abi.array(olds[1])
+    abi.mg_group_norm_bwd(x.ptr, *(v.ptr for v in dev), gy.ptr, gx.ptr, gg.ptr, gb.ptr, n, p, d, 1, K.ACT_RELU, K.ACC_STORE_A)
+    unit = (xv - m4) * r4
+    gz = gv * (unit * gamma + beta > 0)
+    # (all of this is well conditioned: sums of at most 18 000 terms of one size)
+    for got, ref, old, size in ((gg, (gz * unit).sum(axis=(0, 1))[0], olds[0], np.abs(gz * unit).sum(axis=(0, 1))[0]),
+                                (gb, gz.sum(axis=(0, 1))[0], olds[1], np.abs(gz).sum(axis=(0, 1))[0])):
+        assert np.all(np.abs(got.numpy() - (ref + old)) <= 2 * (n * p + 40) * U * (size + np.abs(old)))
+    got = gx.numpy((n, p, 1, d))
+    for i in (0, 1, 7, 8, 295, 296, 4500, n - 1):
+        ref, bound = backward(xv[i:i + 1], gamma, beta, mean[i:i + 1], rstd[i:i + 1], gv[i:i + 1], K.ACT_RELU)
+        near(got[i], ref[0], bound[0])
+    u = gz * gamma
+    full = r4 * (u - u.mean(axis=(1, 3), keepdims=True) - unit * (u * unit).mean(axis=(1, 3), keepdims=True))
+    assert np.abs(got - full).max() <= 1e-11 * np.abs(full).max()
