@@ -8,7 +8,8 @@ import numpy as np
 import pytest
 
 from micrograd_b200 import cabi as K
-from test_gpu_group_norm import backward, call_fwd, near
+from test_gpu_group_norm import backward, call_fwd, make, near, stats
+from test_gpu_linear_xent import problem, reference
 from test_gpu_q8 import Packed, activation, encode
 
 pytestmark = pytest.mark.gpu
@@ -351,3 +352,78 @@ def test_norm_gradients_of_many_wide_rows(abi, p):
     u = gz * gamma
     full = r4 * (u - u.mean(axis=(1, 3), keepdims=True) - unit * (u * unit).mean(axis=(1, 3), keepdims=True))
     assert np.abs(got - full).max() <= 1e-11 * np.abs(full).max()
+
+
+@pytest.mark.parametrize("shifts", [(0, 0, 0), (1, 1, 1), (0, 0, 1), (0, 1, 0), (1, 0, 0)])
+@pytest.mark.parametrize("m", [1, 2, 3, 4])
+def test_few_rows_off_the_vector_boundaries(abi, m, shifts):
+    """Even class counts, whose rows of w and gw are taken in pairs where the addresses of
+    both allow it: x, w and gw start `shifts` doubles behind a boundary."""
+    k, v = 70, 130
+    rng, x, w, b, y = problem(m, k, v, 40 + m, out_rows=0.0)
+    if m > 2:
+        y[1] = -1
+    ref = reference(x, w, b, y, float(m), 0.8)
+    olds = [rng.standard_normal(t.shape) for t in (x, w, b)]
+
+    def put(t, shift):
+        return abi.array(np.concatenate([np.zeros(shift), t.reshape(-1), [55.0]]))
+
+    sx, sw, sg = shifts
+    dx, dw, db, dy, dg, loss = put(x, sx), put(w, sw), abi.array(b), abi.int_array(y), abi.array([0.8]), abi.empty(1)
+    for flags in (0, STORE):
+        out = [put(olds[0], 0), put(olds[1], sg), put(olds[2], 0)]
+        abi.mg_linear_xent_fwd_bwd(dx.offset(sx), dw.offset(sw), db.ptr, dy.ptr, dg.ptr, loss.ptr,
+                                   out[0].ptr, out[1].offset(sg), out[2].ptr, m, k, v, float(m), flags)
+        assert abs(LD(loss.numpy()[0]) - ref["loss"][0]) <= ref["loss"][1]
+        for name, o, old, s in zip(("gx", "gw", "gb"), out, olds, (0, sg, 0)):
+            a = o.numpy()
+            assert a[-1] == 55.0 and not np.any(a[:s])
+            r, bound = ref[name]
+            was = 0 * old if flags else old
+            assert np.all(np.abs(a[s:-1].reshape(old.shape).astype(LD) - (r + was)) <= bound + 2 * U * (np.abs(r) + np.abs(was)))
+    abi.mg_check_kernel_status()
+
+
+@pytest.mark.parametrize("which", ["x", "gy", "gx", "all"])
+@pytest.mark.parametrize("shape", [(9, 3, 4, 8), (5, 1, 3, 64), (3, 50, 2, 12), (2, 6, 1, 4200)])
+def test_norm_gradients_off_the_vector_boundaries(abi, shape, which):
+    """x, gy and gx start one and two doubles behind a 32-byte boundary, one at a time and
+    together, in the warp form (twice), the tile form and the general form."""
+    n, p, g, d = shape
+    rng, x, gamma, beta = make(shape, 41)
+    gy, old = rng.standard_normal(x.shape), rng.standard_normal(x.shape)
+    mean, rstd = (v.astype(np.float64) for v in stats(x, 1e-5))
+    ref, bound = backward(x, gamma, beta, mean, rstd, gy, K.ACT_SILU)
+    params = [abi.array(v) for v in (gamma, beta, mean, rstd)]
+    for shift in (1, 2):
+        s = [shift if which in (name, "all") else 0 for name in ("x", "gy", "gx")]
+        for flags in (0, K.ACC_STORE_A):
+            dx, dgy, dgx = (abi.array(np.concatenate([np.zeros(k), v.reshape(-1), [55.0]])) for k, v in zip(s, (x, gy, old)))
+            gg, gb = abi.empty(g * d), abi.empty(g * d)
+            abi.mg_group_norm_bwd(dx.offset(s[0]), *(v.ptr for v in params), dgy.offset(s[1]), dgx.offset(s[2]), gg.ptr, gb.ptr,
+                                  n, p, g * d, g, K.ACT_SILU, flags | K.ACC_STORE_B | K.ACC_STORE_C)
+            got = dgx.numpy()
+            assert got[-1] == 55.0 and not np.any(got[:s[2]])
+            was = np.zeros(x.size) if flags else old.reshape(-1)
+            near(got[s[2]:-1], ref[0].reshape(-1) + was, bound[0].reshape(-1) + 2 * U * (np.abs(was) + np.abs(ref[0].reshape(-1))))
+            near(gg.numpy(), ref[1], bound[1])
+            near(gb.numpy(), ref[2], bound[2])
+
+
+@pytest.mark.parametrize("shape", [(9, 3, 4, 8), (3, 50, 2, 12)])
+def test_norm_off_the_vector_boundaries(abi, shape):
+    n, p, g, d = shape
+    _, x, gamma, beta = make(shape, 42)
+    want = call_fwd(abi, x, gamma, beta, 1e-5, K.ACT_RELU)
+    dg, db = abi.array(gamma), abi.array(beta)
+    for sx, sy in ((2, 0), (0, 2), (1, 0), (0, 1), (2, 2)):
+        dx = abi.array(np.concatenate([np.zeros(sx), x.reshape(-1)]))
+        y, mean, rstd = abi.array(np.full(sy + x.size + 1, 55.0)), abi.empty(n * g), abi.empty(n * g)
+        abi.mg_group_norm_fwd(dx.offset(sx), dg.ptr, db.ptr, y.offset(sy), mean.ptr, rstd.ptr, n, p, g * d, g, 1e-5, K.ACT_RELU)
+        got = y.numpy()
+        assert got[-1] == 55.0 and np.all(got[:sy] == 55.0)
+        # (another vector width adds the group's values up in another order)
+        e = p * d
+        assert np.abs(got[sy:-1] - want[0]).max() <= 8 * (e + 20) * U * max(1.0, np.abs(x).max()) * want[2].max() * 1.5
+        assert np.abs(mean.numpy() - want[1]).max() <= 2 * e * U * np.abs(x).max()
