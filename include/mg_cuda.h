@@ -242,8 +242,10 @@ int mg_softmax_xent_bwd(const double *logits, const int *labels, const double *g
  * gradient with respect to the loss, each destination may be NULL, and
  * MG_ACC_STORE_A / _B / _C say that gx / gw / gbias hold nothing yet.  The logits
  * exist for a block of rows at a time, in a workspace from the pool of mg_alloc (at
- * most 1 GiB or 16 rows; with up to four rows, M/64 of w's size more for gx).  Any K and V; odd ones, and arrays off a 16-byte boundary,
- * are copied once into rows the tensor kernel can take. */
+ * most 1 GiB or 16 rows; with up to four rows, M/64 of w's size more for gx).  Any K
+ * and V; with more than four rows, w is copied into that workspace where V is odd or w
+ * off a 16-byte boundary (not for the loss alone of up to eight rows), and x where
+ * gradients are wanted, K is odd or x is off one. */
 int mg_linear_xent_fwd(const double *x, const double *w, const double *bias, const int *labels,
                        double *loss1, size_t M, size_t K, size_t V, double denom);
 int mg_linear_xent_fwd_bwd(const double *x, const double *w, const double *bias, const int *labels,

@@ -110,7 +110,8 @@ std::shared_ptr<Tensor> softmax_cross_entropy(const std::shared_ptr<Tensor> &log
 // logits: they exist for a block of rows at a time (at most 1 GiB).  The gradients are
 // computed in the forward pass, which has the block's logits at hand (three products
 // instead of the four that going through them again in the backward pass would take),
-// and kept for backward(); where neither the input nor the head's parameters require a
+// and kept for backward(), which scales them by its own gradient, in buffers of the size
+// of what they belong to, until the graph goes; where neither the input nor the head's parameters require a
 // gradient only the loss is computed (backward() throws std::logic_error for one that
 // came to require a gradient later).  A row with label -1 is left out (a padded
 // batch): it adds nothing to the loss or any gradient, whatever its values are; it does

@@ -369,9 +369,7 @@ add_row_kernel(const double *x, const double *__restrict__ row, double *out, siz
 }
 
 
-// sum() backward: gx[i] += g[0], the scalar read from device memory
-// (src/ops/Reduction.cpp:26-30).  in: old gx.  out: gx.
-// y (+)= a1[0] * x, the factor read on the device.
+// y (+)= a1[0] * x, the factor read on the device.  in: x, old y.  out: y.
 struct ScaleAcc {
   static constexpr int NI = 2, NO = 1;
   const double *in[2];
@@ -382,6 +380,8 @@ struct ScaleAcc {
   }
 };
 
+// sum() backward: gx[i] += g[0], the scalar read from device memory
+// (src/ops/Reduction.cpp:26-30).  in: old gx.  out: gx.
 struct ScalarBroadcastBwd {
   static constexpr int NI = 1, NO = 1;
   const double *in[NI];

@@ -112,12 +112,20 @@ struct NormShape {
   int C, G, D;
 };
 
+// ---------------------------------------------------------------------------
+// General form: what the one-pass forms below do not take, that is groups beyond the
+// shared memory of eight CTAs and rows of more than 512 threads' channels (1024 channels
+// a group in the gradients, 2048 forward; 512 where their number is odd).  x is read two
+// or three times forward (the second time of a piece from L2), and x and gy twice in the
+// gradients: 40 bytes per value.  65 536 x 2048 in one group, SiLU: forward 0.91 ms,
+// gradients 1.79, against 0.33 and 0.49 for what has to be moved.
+// ---------------------------------------------------------------------------
 constexpr int kGnThreads = 256;
-// Values of a group that one CTA takes in the general form: 64 KB, so that its
-// second look at them comes from L2.
+// Values of a group that one CTA takes: 64 KB, so that its second look at them comes
+// from L2.
 constexpr size_t kGnPiece = 8192;
 
-// General form, step 1: moments of one piece of one group.
+// Forward, step 1: moments of one piece of one group.
 __global__ void __launch_bounds__(kGnThreads)
 gn_moments_kernel(const double *__restrict__ x, NormShape s, size_t piece, double *__restrict__ parts,
                   double eps, double *__restrict__ mean_out, double *__restrict__ rstd_out) {
@@ -994,8 +1002,10 @@ static TeamPlan plan_norm(const NormShape &s, uintptr_t address_bits, bool bwd) 
     return t;
   }
   // Backward, four channels' parameters and sums do not fit the registers that 28 warps
-  // per SM leave (128 x 784 x 256 in groups of 8 channels with SiLU: 140 us with 16-byte
-  // cells and 512 threads, 4.4 TB/s; 32-byte cells and 256 threads took 1.3 times as long).
+  // per SM leave (128 x 784 x 256 in groups of 8 channels with SiLU: 144 us with 16-byte
+  // cells and 512 threads, 4.3 TB/s; 32-byte cells and 256 threads took 1.3 times as long).
+  // What holds it there is latency: HBM and the fp64 units are both less than half busy
+  // (48 and 42 %), and the 26 warps of an SM wait for loads and for dependent results.
   // Forward, where less is kept, CTAs of 256 threads are better (103 us; 512 threads: 1.15
   // times as long).
   if (bwd && t.vec > 2) t.vec = 2;

@@ -58,7 +58,8 @@ struct BlockWalk {
 };
 
 // A warp per block, two columns per lane, UN blocks at a time so that 32 to 64 bytes per
-// lane are on their way.  The integer units bound this kernel before HBM does, so the
+// lane are on their way.  The integer units bound this kernel before HBM does (70 and
+// 49 % of their rates at 65 536 x 1024, the fp64 units 19 %), so the
 // block's maximum is taken by two warp-wide integer reductions: of the high words of
 // |x|, then of the low words under the largest high word (their bit patterns are in the
 // order of the values, infinity and NaN above all numbers); and its two quotients are
@@ -461,8 +462,11 @@ static int outer_q8(const double *G, const double *B, double *dA, size_t M, size
 // dB[K][N] (+)= (codes scales)[M][K]^T . G[M][N], N <= 32.  A CTA takes one block of 64
 // columns of the codes (so one scale per row) and a piece of the rows; its four warps
 // take every fourth row, a lane two columns with their N sums each.  The warps' sums are
-// added up in order, the pieces' by a second kernel, in order.  Bound by the fp64 units:
-// N + 2 instructions per code.
+// added up in order, the pieces' by a second kernel, in order.  N + 2 fp64 instructions
+// per code are 43 us of 65 536 x 1024 x 10 at their rate, of 98: the counters show the
+// fp64 units half busy, shared memory at 61 %, 2.1 instructions a cycle from 12 warps per
+// SM.  The rest is what a lane does for a row besides its sums (G's values, a scale, two
+// codes, their widening), which serves two columns only.
 constexpr int kTallThreads = 128, kTallRows = 32;
 // CTAs per SM: 65 536 x 1024, ten columns: 98 us with four and all eight rows of a warp
 // unrolled, 112 with six and two rows (more warps, but twice the instructions a row).
@@ -608,7 +612,6 @@ static int tall_q8(const signed char *codes, const double *scales, const double 
 // x[M][pitch] = the values of codes[M][N]; what is behind the N columns stays as it is.
 static int unpack_rows(const signed char *codes, const double *scales, double *x, size_t pitch, size_t M, size_t N) {
   const size_t nb = q8_blocks(N), blocks = M * nb;
-  cudaStream_t stream = ctx().stream;
   int vec = q8_vec(x, codes, N);
   if (pitch % 4 != 0 && vec == 4) vec = pitch % 2 == 0 ? 2 : 1;
   const unsigned grid = grid_for(blocks * (vec == 4 ? 16 : 32), kQ8Threads, 64);
@@ -647,7 +650,6 @@ int mg_q8_pack(const double *x, signed char *codes, double *scales, size_t M, si
   MG_ENSURE_INIT();
   if (M == 0 || N == 0) return MG_OK;
   const size_t nb = q8_blocks(N), blocks = M * nb;
-  cudaStream_t stream = ctx().stream;
   const unsigned grid = grid_for(blocks * 32, kQ8Threads, 64), wide = (unsigned)nb;
   const bool pair = q8_vec(x, codes, N) >= 2;
   if (pair && N % 64 == 0)
