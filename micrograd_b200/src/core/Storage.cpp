@@ -95,7 +95,7 @@ void Storage::pack8(size_t rows, size_t cols) {
     throw std::logic_error("keep_8bit: the values live in a buffer shared with other tensors");
   }
   const bool recording = mg_graph_recording() != 0;
-  if (dev_in_step_ && mg_graph_count() == 0) {
+  if (dev_in_step_ && !recording && mg_graph_count() == 0) {
     dev_in_step_ = false;  // the steps that used the buffer are gone
   }
   if (codes_) {

@@ -427,3 +427,28 @@ def test_norm_off_the_vector_boundaries(abi, shape):
         e = p * d
         assert np.abs(got[sy:-1] - want[0]).max() <= 8 * (e + 20) * U * max(1.0, np.abs(x).max()) * want[2].max() * 1.5
         assert np.abs(mean.numpy() - want[1]).max() <= 2 * e * U * np.abs(x).max()
+
+
+def test_a_refusal_during_a_recording_forgets_nothing(api, abi):
+    """A tensor that the step being recorded uses is refused then, and afterwards too; the
+    fp64 form of a kept one that it reads stays."""
+    rng = np.random.default_rng(15)
+    x, y = (api.Tensor([6, 70], rng.standard_normal((6, 70))) for _ in range(2))
+    y.keep_8bit()
+    y.add(1.0)  # (its fp64 form)
+
+    def body():
+        out = x.add(1.0), y.add(1.0)
+        with pytest.raises(RuntimeError, match="made before the recording"):
+            x.keep_8bit()
+        y.keep_8bit()
+        return out
+
+    rec, (of_x, of_y) = recorded(api, body)
+    with pytest.raises(RuntimeError, match="a recorded step uses"):
+        x.keep_8bit()
+    y.keep_8bit()
+    filler = [api.Tensor([6, 70], np.full((6, 70), 9.0)) for _ in range(4)]
+    rec.replay()
+    assert np.array_equal(of_x.data(), x.data() + 1.0) and np.array_equal(of_y.data(), y.data() + 1.0) and len(filler) == 4
+    rec.abandon()
