@@ -110,9 +110,10 @@ std::shared_ptr<Tensor> Linear::fused_forward(const std::shared_ptr<Tensor> &inp
     double *masked = nullptr;
     if (relu && !premasked) {
       // dZ = dOut * (out > 0); out > 0 exactly where the pre-activation was.
+      const signed char *own = Access::data(self).packed() ? Access::data(self).codes() : nullptr;
       check(mg_alloc(batch * out, &masked), "device allocation");
-      if (Access::data(self).packed()) {
-        check(mg_relu_bwd_q8(Access::data(self).codes(), g, masked, batch * out, MG_ACC_STORE_A), "relu mask");
+      if (own) {
+        check(mg_relu_bwd_q8(own, g, masked, batch * out, MG_ACC_STORE_A), "relu mask");
       } else {
         check(mg_unary_bwd(MG_RELU, Access::data(self).device_read(), nullptr, 0.0, g, masked,
                            batch * out, MG_ACC_STORE_A),
@@ -121,11 +122,13 @@ std::shared_ptr<Tensor> Linear::fused_forward(const std::shared_ptr<Tensor> &inp
       g = masked;
     }
     bool store = false;
+    // (asked for, and refused, before a gradient is marked as written)
+    const bool reads_x = Access::requires_grad(w) || (Access::requires_grad(x) && Access::is_relu_output(x));
+    const signed char *codes = reads_x && Access::data(x).packed() ? Access::data(x).codes() : nullptr;
     if (Access::requires_grad(w)) {
       double *gw = Access::grad(w).device_accumulate(&store);
-      if (Access::data(x).packed()) {
-        check(mg_gemm_tn_q8(Access::data(x).codes(), Access::data(x).scales(), g, gw, batch, out, in,
-                            store ? 0 : 1),
+      if (codes) {
+        check(mg_gemm_tn_q8(codes, Access::data(x).scales(), g, gw, batch, out, in, store ? 0 : 1),
               "linear dW");
       } else {
         check(mg_gemm_tn(Access::data(x).device_read(), g, gw, batch, out, in, store ? 0 : 1),
@@ -143,9 +146,8 @@ std::shared_ptr<Tensor> Linear::fused_forward(const std::shared_ptr<Tensor> &inp
       const bool mask_input = Access::is_relu_output(x);
       const bool stays_masked = mask_input && Access::grad_fully_masked(x);
       double *gx = Access::grad(x).device_accumulate(&store);
-      if (mask_input && Access::data(x).packed()) {
-        check(mg_gemm_nt_q8(g, Access::data(w).device_read(), gx, batch, out, in, store ? 0 : 1,
-                            Access::data(x).codes()),
+      if (mask_input && codes) {
+        check(mg_gemm_nt_q8(g, Access::data(w).device_read(), gx, batch, out, in, store ? 0 : 1, codes),
               "linear dX");
       } else {
         check(mg_gemm_nt(g, Access::data(w).device_read(), gx, batch, out, in, store ? 0 : 1,

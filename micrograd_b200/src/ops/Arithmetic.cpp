@@ -118,8 +118,9 @@ std::shared_ptr<Tensor> Tensor::unary_op(int op, std::string label, double scala
     const double *g = self.grad_.device_read();
     if (op == MG_RELU && x.data_.packed()) {
       bool store = false;
+      const signed char *codes = x.data_.codes();
       double *gx = x.grad_.device_accumulate(&store);
-      check(mg_relu_bwd_q8(x.data_.codes(), g, gx, self.size(), store ? MG_ACC_STORE_A : 0), "relu backward");
+      check(mg_relu_bwd_q8(codes, g, gx, self.size(), store ? MG_ACC_STORE_A : 0), "relu backward");
       return;
     }
     const double *a = needs_input ? x.data_.device_read() : nullptr;

@@ -37,8 +37,9 @@ std::shared_ptr<Tensor> Tensor::matmul(const std::shared_ptr<Tensor> &b) {
     }
     if (rhs.requires_grad_) {
       if (lhs.data_.packed()) {
+        const signed char *codes = lhs.data_.codes();
         double *gb = rhs.grad_.device_accumulate(&store);
-        check(mg_gemm_tn_q8(lhs.data_.codes(), lhs.data_.scales(), g, gb, m, n, k, store ? 0 : 1), "matmul dB");
+        check(mg_gemm_tn_q8(codes, lhs.data_.scales(), g, gb, m, n, k, store ? 0 : 1), "matmul dB");
         return;
       }
       const double *av = lhs.data_.device_read();

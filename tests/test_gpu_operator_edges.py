@@ -452,3 +452,24 @@ def test_a_refusal_during_a_recording_forgets_nothing(api, abi):
     rec.replay()
     assert np.array_equal(of_x.data(), x.data() + 1.0) and np.array_equal(of_y.data(), y.data() + 1.0) and len(filler) == 4
     rec.abandon()
+
+
+@pytest.mark.parametrize("use", ["product", "mask", "layer"])
+def test_a_refused_gradient_is_not_marked_as_written(api, abi, use):
+    rng = np.random.default_rng(16)
+    t = api.Tensor([12, 70], rng.standard_normal((12, 70)))
+    w = api.Tensor([70, 5], rng.standard_normal((70, 5)))
+    head = api.Linear(70, 5)
+    leaf = {"product": w, "mask": t, "layer": head.weights()}[use]
+    out = t.matmul(w) if use == "product" else t.relu() if use == "mask" else head.forward(t)
+    if use != "mask":
+        t.set_requires_grad(False)
+    loss = out.sum()
+    t.keep_8bit()
+
+    def body():
+        with pytest.raises(RuntimeError, match="other side"):
+            loss.backward()
+
+    recorded(api, body)[0].abandon()
+    assert not np.any(leaf.grad())  # (a logical zero: there is no buffer to read)
